@@ -18,6 +18,7 @@
 #ifndef LANCIUS_CUDA_H
 #define LANCIUS_CUDA_H
 
+#include <stdint.h>
 #include "lancius/lancius_ir.h"
 #include "lancius/lancius_scheduler.h"
 #include "lancius/lancius_memory_planner.h"
@@ -215,6 +216,89 @@ lancius_error lcu_conv2d_bwd(float* out, const float* grad, const float* w, size
 lancius_error lcu_conv2d_bwd_w(float* out, const float* grad, const float* in, size_t N, size_t C_in, size_t H, size_t W,
                                size_t C_out, size_t H_out, size_t W_out, size_t K_h, size_t K_w, size_t stride,
                                size_t pad, void* stream);                                        /* :93-136 */
+
+/* ---- serving: a paged 4-bit key/value cache, attention over it, sampling ------
+ * No counterpart in the reference, whose cache is one contiguous FP64 block per
+ * sequence (kernel_attention_kv_cache above). As with every per-op call, the current
+ * device is the one that the buffers and the stream belong to. None of these calls
+ * allocates or waits, so each can be captured into a CUDA graph; the values in the
+ * device arrays may change between replays, the sizes in the structs may not.
+ *
+ * Cache format: 4-bit codes n = 1 .. 15 for the numbers v = n - 8 in groups of 16 channels
+ * with one e4m3 scale byte each; value = v * scale * unit. Channel 2i of a row is the low
+ * nibble of byte i. scale = e4m3(max|x| / (7 unit)), v = x / (scale * unit), both rounded to the
+ * nearest, ties to even, v held within -7 .. 7. A group that holds a NaN or an infinity gets
+ * the scale NaN (0x7f). Reading takes any code (0 is -8) and any non-negative scale. */
+typedef struct {
+    uint8_t* k_codes;      /* [n_pages][n_heads][page_size][head_dim / 2], 16-byte aligned */
+    uint8_t* v_codes;
+    uint8_t* k_scales;     /* [n_pages][n_heads][page_size][head_dim / 16], 16-byte aligned */
+    uint8_t* v_scales;
+    size_t n_pages;
+    size_t page_size;      /* tokens per page: a power of two, at most 4096 */
+    size_t n_heads;        /* key/value heads */
+    size_t head_dim;       /* 64, 128 or 256 */
+    float k_unit, v_unit;  /* > 0: the size of the values, so that scales fit e4m3 (1 for max|x| in 0.1 .. 3136) */
+} lcu_kv_pages;
+
+/* The sequences that one call works on. Sequence b has seq_len[b] keys, the new tokens of
+ * this step included; key j lies in page page_table[b][j / page_size], slot j % page_size.
+ * The step's tokens are rows token_start[b] .. token_start[b + 1] - 1 of q, k, v and out, in
+ * order, and are the last of the sequence: row token_start[b] + i has position
+ * seq_len[b] - n + i. Rows at and after token_start[n_seqs] belong to no sequence and are
+ * left as they were, as is the cache for them. A token whose position is negative (an idle
+ * slot with seq_len 0) is not appended, and its attention row is zero. */
+typedef struct {
+    const int32_t* page_table;    /* device, [n_seqs][table_width] */
+    size_t table_width;
+    const int32_t* seq_len;       /* device, [n_seqs] */
+    const int32_t* token_start;   /* device, [n_seqs + 1], ascending; NULL: one token per sequence */
+    size_t n_seqs, n_tokens;      /* n_tokens: rows of the token arrays */
+    size_t max_seq_len;           /* host bound of seq_len; 0: table_width * page_size */
+    size_t max_new;               /* host bound of a sequence's new tokens; 0: 1 without token_start, else n_tokens */
+} lcu_kv_batch;
+
+/* Appends the step's keys and values, rotating q and k by their positions on the way
+ * (interleaved pairs as in lcu_rope, angle = position * rope_base^(-2c/head_dim) in 64 bits;
+ * rope_base <= 0: no rotation). Row strides q_ld, k_ld, v_ld in floats, so the three may be
+ * parts of one projection. q_out is [n_tokens][n_q_heads * head_dim] and may be q itself when
+ * q_ld is that width; q_out = q = NULL with n_q_heads = 0 appends only. Two rows of one call
+ * must not share a slot (sequences may share pages that neither appends to). A page number
+ * outside the cache, or a position outside the table or max_seq_len, is not written;
+ * lcu_check_stream then returns LANCIUS_ERROR_SHAPE_MISMATCH. */
+lancius_error lcu_kv_append_paged(const lcu_kv_pages* pages, const lcu_kv_batch* batch, float* q_out, const float* q,
+                                  size_t q_ld, size_t n_q_heads, const float* k, size_t k_ld, const float* v, size_t v_ld,
+                                  double rope_base, void* stream);
+/* The inverse: the cached rows of the step's tokens as FP32, k_out and v_out
+ * [n_tokens][n_heads][head_dim]. With token_start = the running sum of seq_len it reads whole
+ * sequences. A page outside the cache reads as zeros and is reported as above. */
+lancius_error lcu_kv_read_paged(float* k_out, float* v_out, const lcu_kv_pages* pages, const lcu_kv_batch* batch,
+                                void* stream);
+/* out[t][h] = softmax(q[t][h] . K / sqrt(head_dim)) V over keys 0 .. position of row t; query
+ * head h reads key head h / (n_q_heads / n_heads). q rows q_ld floats apart, out
+ * [n_tokens][n_q_heads * head_dim]. workspace: lcu_attention_paged_workspace() bytes, 16-byte
+ * aligned, used by this call alone until it has run (two captured graphs that may run at the
+ * same time need two). A NaN or infinity in the cache shows only in the rows that see it: a
+ * row that sees one in a value is NaN in all its channels. Pages outside the cache count as zeros; they, and
+ * lengths over max_seq_len or max_new, are reported as above (the keys and rows over the
+ * bound are left out). */
+lancius_error lcu_attention_paged(float* out, const float* q, size_t q_ld, size_t n_q_heads, const lcu_kv_pages* pages,
+                                  const lcu_kv_batch* batch, void* workspace, size_t workspace_bytes, void* stream);
+size_t lcu_attention_paged_workspace(const lcu_kv_pages* pages, const lcu_kv_batch* batch, size_t n_q_heads);
+
+/* One token per row of logits [rows][vocab], rows ld floats apart, vocab <= 262144. Per-row
+ * device arrays; a NULL one means 1, off, off, off. With w_i = exp((x_i - max x) / temperature)
+ * and ranks by falling logit, ties by rising index, a row keeps the ranks that pass all of
+ *   rank < top_k (<= 0: off), w_i >= min_p (<= 0: off), and then
+ *   the mass of the ranks before it < top_p * the mass so kept (>= 1: off; rank 0 always stays),
+ * and draws the first index at which the running mass of the kept ones, by rising index,
+ * exceeds u * their mass (u in [0, 1); u >= 1 gives the last kept index). temperature <= 0 or NaN takes
+ * the largest logit, the lowest index among equals. NaN logits count as -infinity; a row that
+ * has nothing above -infinity gives -1. Masses are summed in 64 bits and do not depend on
+ * the order in which the GPU runs. */
+lancius_error lcu_sample(int32_t* token, const float* logits, size_t ld, size_t rows, size_t vocab,
+                         const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                         const float* u, void* stream);
 
 /* Library self-description for tests: the names of this build's kernels. */
 const char* lcu_build_info(void);

@@ -44,6 +44,23 @@ GRAPH_P = C.POINTER(LanciusGraph)
 SCHED_P = C.POINTER(LanciusSchedule)
 PLAN_P = C.POINTER(LanciusPlan)
 
+
+class KvPages(C.Structure):
+    """lcu_kv_pages: the paged 4-bit key/value cache of one layer (device pointers, sizes, units)."""
+    _fields_ = [("k_codes", P), ("v_codes", P), ("k_scales", P), ("v_scales", P), ("n_pages", c_size),
+                ("page_size", c_size), ("n_heads", c_size), ("head_dim", c_size), ("k_unit", C.c_float),
+                ("v_unit", C.c_float)]
+
+
+class KvBatch(C.Structure):
+    """lcu_kv_batch: the sequences that one call on the cache works on."""
+    _fields_ = [("page_table", P), ("table_width", c_size), ("seq_len", P), ("token_start", P), ("n_seqs", c_size),
+                ("n_tokens", c_size), ("max_seq_len", c_size), ("max_new", c_size)]
+
+
+KV_PAGES_P = C.POINTER(KvPages)
+KV_BATCH_P = C.POINTER(KvBatch)
+
 # opcode numbering (lancius_ir.h)
 OPS = ["NOP", "INPUT", "CONST", "ADD", "SUB", "MUL", "MATMUL", "RELU", "SOFTMAX", "SUM", "BROADCAST",
        "TRANSPOSE", "RELU_BWD", "SOFTMAX_BWD", "SUM_AXIS0", "SUM_AXIS1", "CONV2D", "MAXPOOL2D", "FLATTEN",
@@ -160,6 +177,11 @@ B200_FUNCS = {
     "lcu_gqa": (C.c_int, [P, P, P, P, c_size, c_size, c_size, c_size, P]),
     "lcu_attention_kv_cache": (C.c_int, [P, P, P, P, c_size, c_size, c_size, P]),
     "lcu_attention_kv_cache_batched": (C.c_int, [P, P, P, P, c_size, c_size, c_size, c_size, P]),
+    "lcu_kv_append_paged": (C.c_int, [KV_PAGES_P, KV_BATCH_P, P, P, c_size, c_size, P, c_size, P, c_size, C.c_double, P]),
+    "lcu_kv_read_paged": (C.c_int, [P, P, KV_PAGES_P, KV_BATCH_P, P]),
+    "lcu_attention_paged": (C.c_int, [P, P, c_size, c_size, KV_PAGES_P, KV_BATCH_P, P, c_size, P]),
+    "lcu_attention_paged_workspace": (c_size, [KV_PAGES_P, KV_BATCH_P, c_size]),
+    "lcu_sample": (C.c_int, [P, P, c_size, c_size, c_size, P, P, P, P, P, P]),
     "lcu_comm_unique_id": (C.c_int, [P, c_size]),
     "lcu_comm_create": (P, [C.c_int, C.c_int, P, C.c_int]),
     "lcu_comm_destroy": (None, [P]),

@@ -207,13 +207,15 @@ void lcu_ctx_retarget_schedule(lcu_ctx* c, lancius_schedule* s) {
 
 // Waits for `stream`, then reads the tensor-core kernels' watchdog words of the current
 // device (set when a bounded mbarrier wait gave up): any set word is cleared and reported
-// as LANCIUS_ERROR_INTERNAL. The words are per device, shared by every stream on it.
+// as LANCIUS_ERROR_INTERNAL. The last words are the paged cache's (a page number or length out
+// of range), reported as LANCIUS_ERROR_SHAPE_MISMATCH unless a watchdog tripped too. The
+// words are per device, shared by every stream on it.
 lancius_error lcu_check_stream(void* stream) {
     cudaStream_t st = lcu_as_stream(stream);
-    int* words[4] = {lcu_gemm_watchdog_addr(), lcu_attention_watchdog_addr(), lcu_conv_watchdog_addr(),
-                     lcu_int8_watchdog_addr()};
-    int vals[4] = {0, 0, 0, 0};
-    for (int i = 0; i < 4; i++)
+    int* words[6] = {lcu_gemm_watchdog_addr(), lcu_attention_watchdog_addr(), lcu_conv_watchdog_addr(),
+                     lcu_int8_watchdog_addr(), lcu_kv_fault_addr(), lcu_attn_paged_fault_addr()};
+    int vals[6] = {0, 0, 0, 0, 0, 0};
+    for (int i = 0; i < 6; i++)
         if (words[i]) {
             cudaError_t ce = cudaMemcpyAsync(&vals[i], words[i], sizeof(int), cudaMemcpyDeviceToHost, st);
             if (ce != cudaSuccess) return cuda_fail(ce);
@@ -221,14 +223,14 @@ lancius_error lcu_check_stream(void* stream) {
     cudaError_t ce = cudaStreamSynchronize(st);
     if (ce != cudaSuccess) return cuda_fail(ce);
     bool tripped = false;
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < 6; i++)
         if (vals[i] && words[i]) {
-            tripped = true;
+            tripped = tripped || i < 4;
             cudaMemsetAsync(words[i], 0, sizeof(int), st);
         }
-    if (tripped) {
+    if (tripped || vals[4] || vals[5]) {
         cudaStreamSynchronize(st);
-        return fail(LANCIUS_ERROR_INTERNAL);
+        return fail(tripped ? LANCIUS_ERROR_INTERNAL : LANCIUS_ERROR_SHAPE_MISMATCH);
     }
     return LANCIUS_ERROR_OK;
 }

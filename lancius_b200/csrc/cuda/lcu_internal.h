@@ -156,6 +156,9 @@ int* lcu_attention_watchdog_addr(void);
 int* lcu_conv_watchdog_addr(void);
 int* lcu_int8_watchdog_addr(void);
 int* lcu_gemm_watchdog_addr(void);
+// set by the paged-cache kernels when a page number or a length was out of range
+int* lcu_kv_fault_addr(void);
+int* lcu_attn_paged_fault_addr(void);
 void* lcu_scratch_acquire_gather(size_t bytes);
 void* lcu_scratch_acquire_decode(size_t bytes);
 // mode: LCU_MODE_FP32_EXACT (3xTF32) or LCU_MODE_TF32 (one pass)

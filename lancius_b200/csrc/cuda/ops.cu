@@ -104,7 +104,7 @@ lancius_error lcu_conv2d(float* out, const float* in, const float* w, size_t N, 
 }
 
 const char* lcu_build_info(void) {
-    return "lancius_b200 sm_100a: gemm_tcgen05_3xtf32 attention_tcgen05_3xtf32 conv_tcgen05_3xtf32 gemm_simt conv_simt attention_simt layernorm softmax sum_axis1 maxpool eltwise";
+    return "lancius_b200 sm_100a: gemm_tcgen05_3xtf32 attention_tcgen05_3xtf32 conv_tcgen05_3xtf32 gemm_simt conv_simt attention_simt layernorm softmax sum_axis1 maxpool eltwise kv_append_paged kv_read_paged attention_paged sample";
 }
 
 }  // extern "C"
