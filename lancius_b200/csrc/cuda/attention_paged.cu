@@ -1,100 +1,574 @@
 // Attention of a step's tokens over the paged 4-bit cache (lcu_attention_paged).
 //
-// out[t][h] = sum_j p_j V_j, p = softmax(q . K_j / sqrt(D)), j = 0 .. position of row t, as one pass with a
-// running maximum and sum. One CTA per (row, query head); a warp takes every fourth key, its lanes D / 32
-// channels each.
+// out[t][h] = sum_j p_j V_j, p = softmax(q . K_j / sqrt(D)), j = 0 .. position of row t, in one pass over the
+// cache with a running maximum and sum per row.
+//
+// Bound: HBM. A key/value pair of one head is D + D / 8 bytes and is read once for all rows of its key head
+// ((new token, query head) pairs, up to 8 or 16 per CTA); at the measured copy rate an SM receives about 46
+// codes a clock, so turning codes into operands is the work that has to fit beside the loads.
+//
+// Products run as mma.sync m16n8k16 (f16 in, FP32 out). Measured 0.5 of them per clock and SM, each covers 128
+// codes: 64 codes a clock, above the HBM rate. tcgen05 would need the operands written to shared or tensor
+// memory as f16 first, four times the bytes of the codes. The operands are exact: a dequantised value
+// (n - 8) * scale has 8 significant bits, so K and V fit f16 as they are; q (scaled to [1, 2) by a power of two) and p are
+// split into two f16 halves, 22 bits. With at most 8 rows the halves are the two row halves of one MMA (rows
+// 0-7 hi, 8-15 lo, added afterwards); with 9 to 16 rows (WIDE) they are two MMAs.
+//
+// Dequantising: bits 4-7 of each 16-bit half, or'ed with 0x6400, are the f16 number 16 (64 + n); one HFMA2 with
+// (scale / 16, -72 scale) gives (n - 8) scale without rounding. Eight codes take 7 integer and 4 HFMA2
+// instructions. (4-bit floating point needs cvt, measured 25 codes a clock and SM, or as many shifts.)
+//   S = Q K^T: B operand = K^T, whose fragment wants channel pairs of one key: a thread holds D / 4 contiguous
+//     channels of a key, any order of channels will do if q's fragment has the same.
+//   O += P V: B operand = V, whose fragment wants key pairs of one channel: the words of two keys are first
+//     interleaved by 16-bit halves (2 PRMT per 16 codes). S's accumulator layout is P's operand layout.
+//
+// Work: CTA = (chunk of keys, key head, sequence, block of rows), 4 warps that each take every fourth tile of 32
+// keys through a ring of cp.async stages of their own (no block barrier in the loop) and are merged at the end.
+// Shared-memory rows are swizzled in 16-byte pieces so that both fragment reads are free of bank conflicts.
+// Chunks of a sequence are joined by k_attn_paged_join. Rows past a tile's last visible key are filled with
+// zeros by cp.async, so stale bytes never reach an MMA.
 #include "kv_paged.cuh"
 #include <math.h>
 
 namespace {
 
-constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int WARPS = 4, THREADS = 32 * WARPS, TILE = 32;
+constexpr int MAX_CHUNK = 2048;   // keys of a CTA: 512 per warp, so that an FP32 accumulator takes 32 truncated sums
+constexpr float P_BIAS = 7.f;     // p = 2^(s - m + 7): more of the small weights stay above f16's smallest step
+constexpr float RAISE = 8.f;      // the running maximum moves only when exceeded by 2^8: p <= 2^15 fits f16
 
 __device__ int g_attn_paged_fault = 0;
+
+template <int D, bool WIDE>
+struct Shape {
+    static constexpr int ROW = D / 2, SROW = D / 16;            // code and scale bytes of a cached row
+    static constexpr int STAGES = D == 256 ? 2 : D == 128 ? 3 : 4;
+    static constexpr int CODES = TILE * ROW, SCALES = TILE * SROW;
+    static constexpr int STAGE = 2 * (CODES + SCALES);
+    static constexpr int COLS = WIDE ? 16 : 8;                  // rows of q that one CTA serves
+    static constexpr int STEPS = D / 16;
+    static constexpr int Q_BYTES = STEPS * 512 * (WIDE ? 2 : 1);
+    static constexpr int RING = WARPS * STAGES * STAGE;
+    static constexpr int O_LD = D + 4;
+    static constexpr int MERGE = WARPS * COLS * O_LD * 4;       // reuses the ring
+    static constexpr int SMEM = Q_BYTES + (RING > MERGE ? RING : MERGE);
+    static constexpr int RESIDENT = D == 256 ? 2 : D == 128 ? 3 : WIDE ? 4 : 5;   // CTAs per SM that registers and SMEM allow
+};
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool valid) {
+    const int n = valid ? N : 0;
+    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n));
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(N));
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+// codes 0-3 of both 16-bit halves of w -> 4 half2 of (n - 8) * scale; s16 = scale / 16, s72 = -72 * scale
+__device__ __forceinline__ void dequantise(uint32_t w, __half2 s16, __half2 s72, uint32_t (&h)[4]) {
+    constexpr uint32_t M = 0x00f000f0u, BIAS = 0x64006400u;
+    h[0] = as_u32(__hfma2(as_half2(((w << 4) & M) | BIAS), s16, s72));
+    h[1] = as_u32(__hfma2(as_half2((w & M) | BIAS), s16, s72));
+    h[2] = as_u32(__hfma2(as_half2(((w >> 4) & M) | BIAS), s16, s72));
+    h[3] = as_u32(__hfma2(as_half2(((w >> 8) & M) | BIAS), s16, s72));
 }
 
+// byte offset of 16-byte piece c of cached row r in a stage (128-byte lines, pieces permuted per line)
 template <int D>
-__device__ __forceinline__ void row_values(const uint8_t* codes, const uint8_t* scales, long long at, int lane, float (&x)[D / 32]) {
-#pragma unroll
-    for (int i = 0; i < D / 32; i += 2) {
-        const int ch = lane * (D / 32) + i;
-        const uint32_t c = codes[at * (D / 2) + ch / 2];
-        const float sc = kv_scale(scales[at * (D / 16) + ch / 16]);
-        x[i] = (float)((int)(c & 15) - 8) * sc;
-        x[i + 1] = (float)((int)(c >> 4) - 8) * sc;
-    }
+__device__ __forceinline__ int piece(int r, int c) {
+    if (D == 64) { const int line = r >> 2; return line * 128 + ((((r & 3) * 2 + c) ^ ((line & 1) << 1)) << 4); }
+    if (D == 128) { const int line = r >> 1; return line * 128 + ((((r & 1) * 4 + c) ^ ((line & 3) << 1)) << 4); }
+    return r * 128 + ((c ^ ((((r >> 1) & 3) << 1) | (r & 1))) << 4);
 }
 
-template <int D>
-__global__ void __launch_bounds__(THREADS) k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld,
-                                                        int hq, KvPagesDev p, KvBatchDev b, float scale_log2) {
-    constexpr int R = D / 32;
-    __shared__ float sm_m[WARPS], sm_l[WARPS], sm_o[WARPS][D];
-    const int s = blockIdx.z, h = blockIdx.y, i = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// split of p0, p1 into f16 halves
+__device__ __forceinline__ void split(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(p0, p1);
+    const float2 f = __half22float2(h);
+    hi = as_u32(h);
+    lo = as_u32(__floats2half2_rn(p0 - f.x, p1 - f.y));
+}
+
+struct Split { int chunk, splits; };
+
+template <int D, bool WIDE>
+__global__ void __launch_bounds__(THREADS, Shape<D, WIDE>::RESIDENT)
+k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, int hq, KvPagesDev p, KvBatchDev b,
+             float scale_log2, Split sp, float* __restrict__ part_o, float2* __restrict__ part_ml) {
+    using S = Shape<D, WIDE>;
+    constexpr int COLS = S::COLS, R = WIDE ? 2 : 1;   // rows of q per thread
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float col_scale[COLS];
+    __shared__ float sm_m[WARPS][COLS], sm_l[WARPS][COLS];
+    asm volatile("griddepcontrol.launch_dependents;");
+
+    const int group = hq / p.heads, blocks = gridDim.x / sp.splits;
+    const int split_id = blockIdx.x / blocks, block = blockIdx.x % blocks, head = blockIdx.y, s = blockIdx.z;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     int first, count;
     kv_new_tokens(b, s, first, count);
-    if (count > b.max_new && i == 0) g_attn_paged_fault = 1;
-    if (i >= count) return;
-    const int t = first + i, len = b.seq_len[s];
-    int limit = len - (count - i) + 1;   // keys that this row sees
-    if (limit > b.max_len) { limit = b.max_len; g_attn_paged_fault = 1; }
-    const int head = h / (hq / p.heads);
-    float qr[R], o[R], x[R];
+    const int len = b.seq_len[s];
+    const int used = count < b.max_new ? count : b.max_new;       // rows that are computed
+    const int keys = min(max(len, 0), b.max_len);
+    if (split_id == 0 && block == 0 && tid == 0 && (len > b.max_len || count > b.max_new)) g_attn_paged_fault = 1;
+    const int cols = min(COLS, used * group - block * COLS);     // rows of this block
+    const int parts = max(1, (keys + sp.chunk - 1) / sp.chunk);   // chunks of this sequence
+    if (cols <= 0 || split_id >= parts) return;
+
+    // keys that row c of the block sees: those up to its token's position
+    auto limit_of = [&](int c) {
+        const int i = (block * COLS + c) / group;
+        return c < cols ? min(len - (count - i) + 1, b.max_len) : 0;
+    };
+    int limit[R], least = 0x7fffffff;
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        qr[r] = q[(size_t)t * q_ld + (size_t)h * D + lane * R + r] * scale_log2 * p.k_unit;
-        o[r] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    for (int j = warp; j < limit; j += WARPS) {
-        const long long at = kv_row(p, b, s, j, head);
-        if (at < 0) g_attn_paged_fault = 1;
-        float acc = 0.f;
-        if (at >= 0) {
-            row_values<D>(p.k_codes, p.k_scales, at, lane, x);
+    for (int r = 0; r < R; r++) limit[r] = limit_of(g + 8 * r);
+    least = limit_of(0);                                          // positions rise with the row
+    const int begin = split_id * sp.chunk, end = min(begin + sp.chunk, limit_of(cols - 1));
+
+    // loads: tile i of this warp holds keys begin + 32 (warp + 4 i) ...
+    const int tiles_all = end > begin ? (end - begin + TILE - 1) / TILE : 0;
+    const int tiles = tiles_all > warp ? (tiles_all - warp + WARPS - 1) / WARPS : 0;
+    uint8_t* ring = smem + S::Q_BYTES + warp * S::STAGES * S::STAGE;
+    const int32_t* table = b.table + (size_t)s * b.width;
+    const int slot_mask = (1 << p.page_shift) - 1;
+    auto page_of = [&](int i) {   // page of this lane's key of tile i, -1: none
+        const int key = begin + TILE * (warp + WARPS * i) + lane;
+        if (i >= tiles || key >= end) return -1;
+        const int page = table[key >> p.page_shift];
+        if (page >= 0 && page < p.n_pages) return page;
+        g_attn_paged_fault = 1;
+        return -1;
+    };
+    auto issue = [&](int i, int page) {
+        if (i < tiles) {
+            const int key0 = begin + TILE * (warp + WARPS * i);
+            const uint32_t at = smem_u32(ring + (i % S::STAGES) * S::STAGE);
+            constexpr int C = S::ROW / 16, PER = 32 / C;   // pieces of a row, rows per instruction
 #pragma unroll
-            for (int r = 0; r < R; r++) acc = fmaf(qr[r], x[r], acc);
+            for (int it = 0; it < C; it++) {
+                const int r = it * PER + lane / C, c = lane % C;
+                const int pg = __shfl_sync(0xffffffffu, page, r);
+                const size_t row = (((size_t)max(pg, 0) * p.heads + head) << p.page_shift) + ((key0 + r) & slot_mask);
+                const size_t from = row * S::ROW + 16 * c;
+                const uint32_t to = at + piece<D>(r, c);
+                copy_async<16>(to, p.k_codes + from, pg >= 0);
+                copy_async<16>(to + S::CODES, p.v_codes + from, pg >= 0);
+            }
+            const size_t row = (((size_t)max(page, 0) * p.heads + head) << p.page_shift) + ((key0 + lane) & slot_mask);
+            const uint32_t to = at + 2 * S::CODES + lane * S::SROW;
+            copy_async<S::SROW>(to, p.k_scales + row * S::SROW, page >= 0);
+            copy_async<S::SROW>(to + S::SCALES, p.v_scales + row * S::SROW, page >= 0);
         }
-        acc = warp_sum(acc);
-        const float mx = fmaxf(m, acc), corr = m == -INFINITY ? 0.f : ex2(m - mx), pj = ex2(acc - mx);
+        asm volatile("cp.async.commit_group;");
+    };
+    int page_next[S::STAGES];
 #pragma unroll
-        for (int r = 0; r < R; r++) x[r] = 0.f;
-        if (at >= 0) row_values<D>(p.v_codes, p.v_scales, at, lane, x);
-        bool nan = false;
+    for (int i = 0; i < S::STAGES; i++) page_next[i] = page_of(i);
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; i++) issue(i, page_next[i]);
+    int page_ahead = page_next[S::STAGES - 1];
+
+    // q as A fragments in shared memory: [step][lane][4], rows 0-7 / 8-15 = hi / lo halves of 8 rows, or (WIDE) 16 rows,
+    // hi fragments first, then lo
+    for (int c = warp; c < COLS; c += WARPS) {
+        constexpr int N = D / 32;
+        const int ci = block * COLS + c;
+        float x[N], amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            x[i] = c < cols ? q[(size_t)(first + ci / group) * q_ld + (size_t)(head * group + ci % group) * D + lane + 32 * i] : 0.f;
+            amax = fmaxf(amax, fabsf(x[i]));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        int e = (int)(__float_as_uint(amax) >> 23) - 127;          // 2^e <= amax < 2^(e + 1)
+        if (amax == 0.f || e > 127) e = 0;
+        e = min(max(e, -126), 126);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+        if (lane == 0) col_scale[c] = scale_log2 * p.k_unit * up;
+        __half* frag = reinterpret_cast<__half*>(smem);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int ch = lane + 32 * i, owner = ch / (D / 4), in = ch % (D / 4), step = in / 8 * 2 + ((in & 3) >> 1);
+            const float y = x[i] * down;
+            const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
+            const int at = ((step * 32 + (c & 7) * 4 + owner) * 4 + (in & 1) * 2) * 2 + ((in >> 2) & 1);   // register 0 or 2
+            if (WIDE) {
+                frag[at + (c >> 3) * 2] = hi;
+                frag[at + (c >> 3) * 2 + S::STEPS * 256] = lo;
+            } else {
+                frag[at] = hi;
+                frag[at + 2] = lo;
+            }
+        }
+    }
+    __syncthreads();
+
+    float o[D / 8][4], m[R], l[R], cs[R];
+#pragma unroll
+    for (int j = 0; j < D / 8; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) o[j][r] = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; r++) { m[r] = -INFINITY; l[r] = 0.f; cs[r] = col_scale[g + 8 * r]; }
+    const uint4* q_frag = reinterpret_cast<const uint4*>(smem) + lane;
+    const __half2 inv16 = __float2half2_rn(0.0625f), neg72 = __float2half2_rn(-72.f);
+
+    for (int i = 0; i < tiles; i++) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2));
+        __syncwarp();   // the tile is there for all lanes, and the stage before it is free
+        issue(i + S::STAGES - 1, page_ahead);
+        page_ahead = page_of(i + S::STAGES);
+        const uint8_t* st = ring + (i % S::STAGES) * S::STAGE;
+        const int key0 = begin + TILE * (warp + WARPS * i);
+
+        // ---- S = Q K^T, 8 keys at a time
+        float a[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            const int r = n * 8 + g;
+            uint32_t w[D / 32];
+            if constexpr (D == 64) {
+                const uint2 v = *reinterpret_cast<const uint2*>(st + piece<D>(r, t >> 1) + (t & 1) * 8);
+                w[0] = v.x; w[1] = v.y;
+            } else {
+#pragma unroll
+                for (int c = 0; c < D / 128; c++) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(st + piece<D>(r, t * (D / 128) + c));
+                    w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
+                }
+            }
+            const uint8_t* sc = st + 2 * S::CODES + r * S::SROW + t * (D / 64);
+            uint32_t sw[D == 256 ? 2 : 1];   // pairs of scales
+            if constexpr (D == 64) sw[0] = *sc;
+            else if constexpr (D == 128) sw[0] = *reinterpret_cast<const uint16_t*>(sc);
+            else { const uint32_t v = *reinterpret_cast<const uint32_t*>(sc); sw[0] = v & 0xffff; sw[1] = v >> 16; }
+#pragma unroll
+            for (int r4 = 0; r4 < 4; r4++) a[n][r4] = 0.f;
+#pragma unroll
+            for (int wi = 0; wi < D / 32; wi++) {
+                const __half2 two = as_half2(kv_scales_to_half(sw[wi / 4]));
+                const __half2 one = (wi / 2) & 1 ? __high2half2(two) : __low2half2(two);
+                uint32_t h[4];
+                dequantise(w[wi], __hmul2(one, inv16), __hmul2(one, neg72), h);
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const uint4 f = q_frag[(2 * wi + u) * 32];
+                    const uint32_t qa[4] = {f.x, f.y, f.z, f.w};
+                    mma(a[n], qa, h[2 * u], h[2 * u + 1]);
+                    if (WIDE) {
+                        const uint4 f2 = q_frag[(S::STEPS + 2 * wi + u) * 32];
+                        const uint32_t ql[4] = {f2.x, f2.y, f2.z, f2.w};
+                        mma(a[n], ql, h[2 * u], h[2 * u + 1]);
+                    }
+                }
+            }
+        }
+
+        // ---- V's scales: bytes of keys 2t, 2t + 1, 2t + 8, 2t + 9 of each 16-key half, this thread's channel groups
+        constexpr int VG = D == 256 ? 2 : 1;
+        uint32_t vs[2][VG];
+        uint32_t nan = 0;
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
+            const uint8_t* sc = st + 2 * S::CODES + S::SCALES + (16 * kb + 2 * t) * S::SROW + (D == 64 ? g >> 1 : g * VG);
+#pragma unroll
+            for (int x = 0; x < VG; x++) {
+                vs[kb][x] = (uint32_t)sc[x] | (uint32_t)sc[S::SROW + x] << 8 | (uint32_t)sc[8 * S::SROW + x] << 16 |
+                            (uint32_t)sc[9 * S::SROW + x] << 24;
+                nan |= (vs[kb][x] + 0x01010101u) & 0x80808080u;
+            }
+        }
+        // A NaN in a value must not meet the zero weights of rows that do not see it: its scale becomes 0 and the
+        // weights of the rows that see it become NaN.
+        uint32_t poison = 0;   // keys of the tile
+        if (__any_sync(0xffffffffu, nan)) {
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int x = 0; x < VG; x++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+                        if ((vs[kb][x] >> (8 * y) & 0x7f) == 0x7f) {
+                            vs[kb][x] &= ~(0xffu << (8 * y));
+                            poison |= 1u << (16 * kb + 2 * t + (y & 1) + (y >> 1) * 8);
+                        }
+            poison = __reduce_or_sync(0xffffffffu, poison);
+        }
+
+        // ---- weights
+        float sv[R][8], top[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            nan = nan || x[r] != x[r];
-            o[r] = fmaf(pj, x[r], o[r] * corr);
+            top[r] = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    float x = WIDE ? a[n][2 * r + u] : a[n][u] + a[n][2 + u];
+                    x *= cs[r];
+                    sv[r][2 * n + u] = x;
+                }
         }
-        l = l * corr + pj;
-        if (__any_sync(0xffffffffu, nan)) l = NAN;
+        if (key0 + TILE > least) {
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int x = 0; x < 8; x++)
+                    if (key0 + (x >> 1) * 8 + 2 * t + (x & 1) >= limit[r]) sv[r][x] = -INFINITY;
+        }
+        bool raise = false;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+#pragma unroll
+            for (int x = 0; x < 8; x++) top[r] = fmaxf(top[r], sv[r][x]);
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+            raise = raise || top[r] > m[r] + RAISE;
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+            float f[R];
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const float mx = fmaxf(m[r], top[r]);
+                f[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - mx);   // nothing was summed before the first key
+                m[r] = mx;
+                l[r] *= f[r];
+            }
+#pragma unroll
+            for (int j = 0; j < D / 8; j++) {
+                o[j][0] *= f[0]; o[j][1] *= f[0];
+                o[j][2] *= f[R - 1]; o[j][3] *= f[R - 1];
+            }
+        }
+        uint32_t hi[R][4], lo[R][4];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const float base = m[r] == -INFINITY ? 0.f : m[r] - P_BIAS;
+            float pw[8];
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                pw[x] = ex2(sv[r][x] - base);
+                if (poison) {
+                    const int k = (x >> 1) * 8 + 2 * t + (x & 1);
+                    if ((poison >> k & 1) && key0 + k < limit[r]) pw[x] = NAN;
+                }
+                l[r] += pw[x];
+            }
+#pragma unroll
+            for (int n = 0; n < 4; n++) split(pw[2 * n], pw[2 * n + 1], hi[r][n], lo[r][n]);
+        }
+
+        // ---- O += P V, 16 keys at a time
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
+            const uint8_t* vt = st + S::CODES;
+            uint32_t w[4][D / 64];   // keys 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const int r = 16 * kb + 2 * t + (y & 1) + (y >> 1) * 8;
+                if constexpr (D == 64) {
+                    w[y][0] = *reinterpret_cast<const uint32_t*>(vt + piece<D>(r, g >> 2) + (g & 3) * 4);
+                } else if constexpr (D == 128) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(vt + piece<D>(r, g >> 1) + (g & 1) * 8);
+                    w[y][0] = v.x; w[y][1] = v.y;
+                } else {
+                    const uint4 v = *reinterpret_cast<const uint4*>(vt + piece<D>(r, g));
+                    w[y][0] = v.x; w[y][1] = v.y; w[y][2] = v.z; w[y][3] = v.w;
+                }
+            }
+            const uint32_t pa[4] = {hi[0][2 * kb], WIDE ? hi[R - 1][2 * kb] : lo[0][2 * kb], hi[0][2 * kb + 1],
+                                    WIDE ? hi[R - 1][2 * kb + 1] : lo[0][2 * kb + 1]};
+            const uint32_t pl[4] = {lo[0][2 * kb], lo[R - 1][2 * kb], lo[0][2 * kb + 1], lo[R - 1][2 * kb + 1]};
+#pragma unroll
+            for (int wi = 0; wi < D / 64; wi++) {
+                const uint32_t sc = vs[kb][wi / 2 % VG];
+                const __half2 sa = as_half2(kv_scales_to_half(sc & 0xffff)), sb = as_half2(kv_scales_to_half(sc >> 16));
+                const __half2 a16 = __hmul2(sa, inv16), a72 = __hmul2(sa, neg72), b16 = __hmul2(sb, inv16), b72 = __hmul2(sb, neg72);
+#pragma unroll
+                for (int half = 0; half < 2; half++) {   // channels 0-3, 4-7 of the words
+                    const uint32_t sel = half ? 0x7632 : 0x5410;
+                    uint32_t h0[4], h1[4];
+                    dequantise(__byte_perm(w[0][wi], w[1][wi], sel), a16, a72, h0);
+                    dequantise(__byte_perm(w[2][wi], w[3][wi], sel), b16, b72, h1);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        mma(o[8 * wi + 4 * half + j], pa, h0[j], h1[j]);
+                        if (WIDE) mma(o[8 * wi + 4 * half + j], pl, h0[j], h1[j]);
+                    }
+                }
+            }
+        }
+    }
+    asm volatile("cp.async.wait_all;");
+
+    // ---- merge the warps. Thread (g, t) holds channels 2t D/8 + j and (2t + 1) D/8 + j of its rows.
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        if (t == 0) { sm_m[warp][g + 8 * r] = m[r]; sm_l[warp][g + 8 * r] = l[r]; }
+    }
+    __syncthreads();   // every ring is idle
+    float* so = reinterpret_cast<float*>(smem + S::Q_BYTES);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        float* at = so + (warp * COLS + g + 8 * r) * S::O_LD + 2 * t * (D / 8);
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int j = 0; j < D / 8; j += 4) {
+                auto v = [&](int x) { return WIDE ? o[j + x][2 * r + u] : o[j + x][u] + o[j + x][2 + u]; };
+                *reinterpret_cast<float4*>(at + u * (D / 8) + j) = make_float4(v(0), v(1), v(2), v(3));
+            }
+    }
+    __syncthreads();
+    for (int x = tid; x < cols * (D / 4); x += THREADS) {
+        const int c = x / (D / 4), d = x % (D / 4) * 4, ci = block * COLS + c;
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) M = fmaxf(M, sm_m[w][c]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+            // a warp without a key has l = 0, or NaN where every score it saw was NaN
+            const float f = sm_m[w][c] == -INFINITY ? 1.f : ex2(sm_m[w][c] - M);
+            L += f * sm_l[w][c];
+            const float4 v = *reinterpret_cast<const float4*>(so + (w * COLS + c) * S::O_LD + d);
+            acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+        }
+        const size_t row = (size_t)(first + ci / group) * hq + head * group + ci % group;
+        if (parts == 1) {
+            const float inv = L == 0.f ? 0.f : p.v_unit / L;
+            float* dst = out + row * D + d;
+            dst[0] = acc.x * inv; dst[1] = acc.y * inv; dst[2] = acc.z * inv; dst[3] = acc.w * inv;
+        } else {
+            const size_t at = row * sp.splits + split_id;
+            *reinterpret_cast<float4*>(part_o + at * D + d) = acc;
+            if (d == 0) part_ml[at] = make_float2(M, L);
+        }
+    }
+}
+
+// out row = sum over its chunks of 2^(m - M) o / sum of 2^(m - M) l; one CTA per row, a warp per fourth chunk
+template <int D>
+__global__ void __launch_bounds__(THREADS) k_attn_paged_join(float* __restrict__ out, int hq, KvBatchDev b, float v_unit, Split sp,
+                                                             const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
+    constexpr int N = D / 32;
+    __shared__ float sm_l[WARPS], sm_m[WARPS];
+    __shared__ float sm_o[WARPS][D];
+    const int s = blockIdx.z, i = blockIdx.y, h = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int first, count;
+    kv_new_tokens(b, s, first, count);
+    const int keys = min(max(b.seq_len[s], 0), b.max_len), parts = (keys + sp.chunk - 1) / sp.chunk;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // also before an early return: the next kernel waits for this one only
+    if (i >= count || parts <= 1) return;
+    const size_t row = (size_t)(first + i) * hq + h;
+    float m = -INFINITY, l = 0.f, o[N];
+#pragma unroll
+    for (int n = 0; n < N; n++) o[n] = 0.f;
+    for (int c = warp; c < parts; c += WARPS) {
+        const float2 ml = part_ml[row * sp.splits + c];
+        const float* po = part_o + (row * sp.splits + c) * D + lane;
+        const float mx = fmaxf(m, ml.x);
+        const float old = m == -INFINITY ? 1.f : ex2(m - mx), f = ml.x == -INFINITY ? 1.f : ex2(ml.x - mx);
+        l = l * old + ml.y * f;
+#pragma unroll
+        for (int n = 0; n < N; n++) o[n] = o[n] * old + po[32 * n] * f;
         m = mx;
     }
     if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
 #pragma unroll
-    for (int r = 0; r < R; r++) sm_o[warp][lane * R + r] = o[r];
+    for (int n = 0; n < N; n++) sm_o[warp][lane + 32 * n] = o[n];
     __syncthreads();
     float M = -INFINITY, L = 0.f;
+#pragma unroll
     for (int w = 0; w < WARPS; w++) M = fmaxf(M, sm_m[w]);
-    for (int w = 0; w < WARPS; w++) L += sm_m[w] == -INFINITY && sm_l[w] == 0.f ? 0.f : ex2(sm_m[w] - M) * sm_l[w];
+    float f[WARPS];
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+        f[w] = sm_m[w] == -INFINITY ? 1.f : ex2(sm_m[w] - M);
+        L += f[w] * sm_l[w];
+    }
+    const float inv = L == 0.f ? 0.f : v_unit / L;
     for (int d = threadIdx.x; d < D; d += THREADS) {
         float acc = 0.f;
-        for (int w = 0; w < WARPS; w++) acc += sm_m[w] == -INFINITY && sm_l[w] == 0.f ? 0.f : ex2(sm_m[w] - M) * sm_o[w][d];
-        out[(size_t)t * hq * D + (size_t)h * D + d] = limit > 0 ? acc / L * p.v_unit : 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) acc += f[w] * sm_o[w][d];
+        out[row * D + d] = acc * inv;
     }
 }
 
 lancius_error bad(lancius_error e) { lancius_set_error(e); return e; }
+
+int row_blocks(int rows) { return rows > 8 ? (rows + 15) / 16 : 1; }
+
+// Chunks: about two rounds of the CTAs that fit on the GPU (a longer chunk wastes the end of the last round, a shorter
+// one spends more on its start and on joining), a multiple of one tile per warp.
+Split plan(const KvPagesDev& p, const KvBatchDev& b, int D, int group) {
+    const int per_sm = D == 256 ? Shape<256, false>::RESIDENT : D == 128 ? Shape<128, false>::RESIDENT : Shape<64, false>::RESIDENT;
+    const size_t ctas = (size_t)b.n_seqs * p.heads * row_blocks(group * b.max_new), len = b.max_len > 0 ? b.max_len : 1;
+    const size_t slots = 2 * (size_t)LCU_SMS * per_sm;
+    size_t chunk = (len * ctas + slots - 1) / slots;
+    constexpr size_t STEP = TILE * WARPS;
+    chunk = (chunk + STEP - 1) / STEP * STEP;
+    if (chunk < STEP) chunk = STEP;
+    if (chunk > MAX_CHUNK) chunk = MAX_CHUNK;
+    return Split{(int)chunk, (int)((len + chunk - 1) / chunk)};
+}
+size_t part_rows(const KvBatchDev& b, size_t hq, Split sp) { return (size_t)b.n_tokens * hq * sp.splits; }
+
+lancius_error check_call(const lcu_kv_pages* pages, const lcu_kv_batch* batch, size_t n_q_heads, KvPagesDev* p, KvBatchDev* b) {
+    lancius_error e = lcu_kv_describe(pages, batch, p, b);
+    if (e != LANCIUS_ERROR_OK) return e;
+    const size_t rows = n_q_heads / pages->n_heads * b->max_new;
+    if (n_q_heads > 65535 || n_q_heads % pages->n_heads || b->max_new > 65535 || rows > (size_t)INT32_MAX / 2)
+        return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
+    return LANCIUS_ERROR_OK;
+}
+
+template <int D, bool WIDE>
+lancius_error launch(float* out, const float* q, size_t q_ld, int hq, const KvPagesDev& p, const KvBatchDev& b, Split sp,
+                     float* part_o, float2* part_ml, cudaStream_t st) {
+    using S = Shape<D, WIDE>;
+    cudaError_t ce = cudaFuncSetAttribute(k_attn_paged<D, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (ce != cudaSuccess) return lcu_check_cuda(ce);
+    const dim3 grid((unsigned)(sp.splits * row_blocks(hq / p.heads * b.max_new)), (unsigned)p.heads, (unsigned)b.n_seqs);
+    k_attn_paged<D, WIDE><<<grid, THREADS, S::SMEM, st>>>(out, q, q_ld, hq, p, b, (float)(1.4426950408889634 / sqrt((double)D)), sp,
+                                                          part_o, part_ml);
+    lcu_note_launch();
+    if (sp.splits == 1) return lcu_launch_status();
+    ce = cudaGetLastError();
+    if (ce != cudaSuccess) return lcu_check_cuda(ce);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // starts while the chunks finish
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)hq, (unsigned)b.max_new, (unsigned)b.n_seqs);
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    ce = cudaLaunchKernelEx(&cfg, k_attn_paged_join<D>, out, hq, b, p.v_unit, sp, (const float*)part_o, (const float2*)part_ml);
+    if (ce != cudaSuccess) {
+        cudaGetLastError();
+        return lcu_check_cuda(ce);
+    }
+    lcu_note_launch();
+    return lcu_launch_status();
+}
 
 }  // namespace
 
@@ -106,30 +580,43 @@ int* lcu_attn_paged_fault_addr(void) {
 }
 
 size_t lcu_attention_paged_workspace(const lcu_kv_pages* pages, const lcu_kv_batch* batch, size_t n_q_heads) {
-    (void)pages; (void)batch; (void)n_q_heads;
-    return 0;
+    KvPagesDev p;
+    KvBatchDev b;
+    if (check_call(pages, batch, n_q_heads, &p, &b) != LANCIUS_ERROR_OK || !b.n_seqs || !b.n_tokens || !n_q_heads) return 0;
+    const Split sp = plan(p, b, (int)pages->head_dim, (int)(n_q_heads / pages->n_heads));
+    return sp.splits == 1 ? 0 : part_rows(b, n_q_heads, sp) * (pages->head_dim + 2) * sizeof(float);
 }
 
 lancius_error lcu_attention_paged(float* out, const float* q, size_t q_ld, size_t n_q_heads, const lcu_kv_pages* pages,
                                   const lcu_kv_batch* batch, void* workspace, size_t workspace_bytes, void* stream) {
     KvPagesDev p;
     KvBatchDev b;
-    lancius_error e = lcu_kv_describe(pages, batch, &p, &b);
+    lancius_error e = check_call(pages, batch, n_q_heads, &p, &b);
     if (e != LANCIUS_ERROR_OK) return e;
     if (!b.n_seqs || !b.n_tokens || !n_q_heads) return LANCIUS_ERROR_OK;
     if (!out || !q) return bad(LANCIUS_ERROR_NULL_PTR);
     const size_t D = pages->head_dim;
-    if (n_q_heads > 65535 || n_q_heads % pages->n_heads || q_ld < n_q_heads * D) return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
-    const float scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
-    const dim3 grid((unsigned)b.max_new, (unsigned)n_q_heads, (unsigned)b.n_seqs);
-    cudaStream_t st = lcu_as_stream(stream);
+    if (q_ld < n_q_heads * D) return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
     const int hq = (int)n_q_heads;
-    if (D == 64) k_attn_paged<64><<<grid, THREADS, 0, st>>>(out, q, q_ld, hq, p, b, scale_log2);
-    else if (D == 128) k_attn_paged<128><<<grid, THREADS, 0, st>>>(out, q, q_ld, hq, p, b, scale_log2);
-    else k_attn_paged<256><<<grid, THREADS, 0, st>>>(out, q, q_ld, hq, p, b, scale_log2);
-    (void)workspace; (void)workspace_bytes;
-    lcu_note_launch();
-    return lcu_launch_status();
+    const Split sp = plan(p, b, (int)D, hq / p.heads);
+    float* part_o = nullptr;
+    float2* part_ml = nullptr;
+    if (sp.splits > 1) {
+        const size_t rows = part_rows(b, n_q_heads, sp);
+        if (!workspace) return bad(LANCIUS_ERROR_NULL_PTR);
+        if ((uintptr_t)workspace & 15u) return bad(LANCIUS_ERROR_UNSUPPORTED_DTYPE);
+        if (workspace_bytes < rows * (D + 2) * sizeof(float)) return bad(LANCIUS_ERROR_OVERFLOW);
+        part_o = static_cast<float*>(workspace);
+        part_ml = reinterpret_cast<float2*>(part_o + rows * D);
+    }
+    const bool wide = hq / p.heads * b.max_new > 8;   // more rows than one MMA's hi/lo halves hold
+    cudaStream_t st = lcu_as_stream(stream);
+    if (D == 64) return wide ? launch<64, true>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st)
+                             : launch<64, false>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
+    if (D == 128) return wide ? launch<128, true>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st)
+                              : launch<128, false>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
+    return wide ? launch<256, true>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st)
+                : launch<256, false>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
 }
 
 }  // extern "C"

@@ -17,8 +17,7 @@ struct KvBatchDev {
 // Checks both descriptions and fills the device forms (max_len, max_new resolved).
 lancius_error lcu_kv_describe(const lcu_kv_pages* pages, const lcu_kv_batch* batch, KvPagesDev* p, KvBatchDev* b);
 
-// First row and number of new tokens of sequence s, clipped to the token arrays. A number over
-// max_new keeps its LAST max_new rows out of reach (bad is set; the caller reports it).
+// First row and number of new tokens of sequence s, clipped to the token arrays.
 __device__ __forceinline__ void kv_new_tokens(const KvBatchDev& b, int s, int& first, int& count) {
     first = b.start ? b.start[s] : s;
     int end = b.start ? b.start[s + 1] : s + 1;
