@@ -14,9 +14,9 @@
 // split into two f16 halves, 22 bits. With at most 8 rows the halves are the two row halves of one MMA (rows
 // 0-7 hi, 8-15 lo, added afterwards); with 9 to 16 rows (WIDE) they are two MMAs.
 //
-// Dequantising: bits 4-7 of each 16-bit half, or'ed with 0x6400, are the f16 number 16 (64 + n); one HFMA2 with
-// (scale / 16, -72 scale) gives (n - 8) scale without rounding. Eight codes take 7 integer and 4 HFMA2
-// instructions. (4-bit floating point needs cvt, measured 25 codes a clock and SM, or as many shifts.)
+// Dequantising: a code or'ed into the mantissa of an f16 constant, then one HFMA2 with the group's factor and offset
+// gives (n - 8) scale / 16 without rounding (scale_of). Eight codes take 5 integer and 4 HFMA2 instructions. (4-bit
+// floating point needs cvt, measured 25 codes a clock and SM, or more shifts.)
 //   S = Q K^T: B operand = K^T, whose fragment wants channel pairs of one key: a thread holds D / 4 contiguous
 //     channels of a key, any order of channels will do if q's fragment has the same.
 //   O += P V: B operand = V, whose fragment wants key pairs of one channel: the words of two keys are first
@@ -35,6 +35,7 @@ namespace {
 constexpr int WARPS = 4, THREADS = 32 * WARPS, TILE = 32;
 constexpr int MAX_CHUNK = 2048;   // keys of a CTA: 512 per warp, so that an FP32 accumulator takes 32 truncated sums
 constexpr float P_BIAS = 7.f;     // p = 2^(s - m + 7): more of the small weights stay above f16's smallest step
+constexpr uint32_t NONE = 0xffffffffu;
 constexpr float RAISE = 8.f;      // the running maximum moves only when exceeded by 2^8: p <= 2^15 fits f16
 
 __device__ int g_attn_paged_fault = 0;
@@ -75,13 +76,30 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-// codes 0-3 of both 16-bit halves of w -> 4 half2 of (n - 8) * scale; s16 = scale / 16, s72 = -72 * scale
-__device__ __forceinline__ void dequantise(uint32_t w, __half2 s16, __half2 s72, uint32_t (&h)[4]) {
-    constexpr uint32_t M = 0x00f000f0u, BIAS = 0x64006400u;
-    h[0] = as_u32(__hfma2(as_half2(((w << 4) & M) | BIAS), s16, s72));
-    h[1] = as_u32(__hfma2(as_half2((w & M) | BIAS), s16, s72));
-    h[2] = as_u32(__hfma2(as_half2(((w >> 4) & M) | BIAS), s16, s72));
-    h[3] = as_u32(__hfma2(as_half2(((w >> 8) & M) | BIAS), s16, s72));
+// A group's scale s (in both halves of `two`) as the factors and offsets of its codes: codes in bits 0-3 of a 16-bit
+// half, or'ed with 0x6400, are the f16 number 1024 + n, those in bits 4-7 are 16 (64 + n). All are exact: s has 4
+// significant bits, 129 * 15 < 2^11. Values come out as (n - 8) s / 16, so that 64.5 s stays below f16's largest.
+struct Scale { __half2 m0, b0, m4, b4; };
+__device__ __forceinline__ Scale scale_of(uint32_t two) {
+    const __half2 s = as_half2(two);
+    return Scale{__hmul2(s, __float2half2_rn(0.0625f)), __hmul2(s, __float2half2_rn(-64.5f)),
+                 __hmul2(s, __float2half2_rn(0.00390625f)), __hmul2(s, __float2half2_rn(-4.5f))};
+}
+// The masks are held in registers that the compiler cannot see through: (w & mask) | bias with two immediates would
+// take two LOP3, and these are the instructions that the kernel executes most.
+struct Masks { uint32_t m0, m4; };
+__device__ __forceinline__ uint32_t code_bits(uint32_t w, uint32_t mask) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, 0x64006400, 0xea;" : "=r"(r) : "r"(w), "r"(mask));
+    return r;
+}
+// the 4 codes of both 16-bit halves of w -> 4 half2
+__device__ __forceinline__ void dequantise(uint32_t w, const Scale& s, const Masks& k, uint32_t (&h)[4]) {
+    const uint32_t v = w >> 8;
+    h[0] = as_u32(__hfma2(as_half2(code_bits(w, k.m0)), s.m0, s.b0));
+    h[1] = as_u32(__hfma2(as_half2(code_bits(w, k.m4)), s.m4, s.b4));
+    h[2] = as_u32(__hfma2(as_half2(code_bits(v, k.m0)), s.m0, s.b0));
+    h[3] = as_u32(__hfma2(as_half2(code_bits(v, k.m4)), s.m4, s.b4));
 }
 
 // byte offset of 16-byte piece c of cached row r in a stage (128-byte lines, pieces permuted per line)
@@ -113,6 +131,8 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     __shared__ float sm_m[WARPS][COLS], sm_l[WARPS][COLS];
     asm volatile("griddepcontrol.launch_dependents;");
 
+    const uint32_t zero = (uint32_t)p.heads >> 31;
+    const Masks masks{0x000f000fu + zero, 0x00f000f0u + zero};
     const int group = hq / p.heads, blocks = gridDim.x / sp.splits;
     const int split_id = blockIdx.x / blocks, block = blockIdx.x % blocks, head = blockIdx.y, s = blockIdx.z;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -143,42 +163,45 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     uint8_t* ring = smem + S::Q_BYTES + warp * S::STAGES * S::STAGE;
     const int32_t* table = b.table + (size_t)s * b.width;
     const int slot_mask = (1 << p.page_shift) - 1;
-    auto page_of = [&](int i) {   // page of this lane's key of tile i, -1: none
+    const uint32_t heads = p.heads;
+    auto row_of = [&](int i) {   // cache row of this lane's key of tile i, NONE: no key, or no such page
         const int key = begin + TILE * (warp + WARPS * i) + lane;
-        if (i >= tiles || key >= end) return -1;
+        if (i >= tiles || key >= end) return NONE;
         const int page = table[key >> p.page_shift];
-        if (page >= 0 && page < p.n_pages) return page;
+        if (page >= 0 && page < p.n_pages) return (((uint32_t)page * heads + head) << p.page_shift) + (key & slot_mask);
         g_attn_paged_fault = 1;
-        return -1;
+        return NONE;
     };
-    auto issue = [&](int i, int page) {
-        if (i < tiles) {
-            const int key0 = begin + TILE * (warp + WARPS * i);
-            const uint32_t at = smem_u32(ring + (i % S::STAGES) * S::STAGE);
-            constexpr int C = S::ROW / 16, PER = 32 / C;   // pieces of a row, rows per instruction
+    // a row's pieces are copied by neighbouring lanes, PER rows an instruction
+    constexpr int C = S::ROW / 16, PER = 32 / C;
+    const uint8_t* k_from = p.k_codes + 16 * (lane % C);
+    const uint8_t* v_from = p.v_codes + 16 * (lane % C);
+    const uint32_t ring_at = smem_u32(ring), piece_at = piece<D>(lane / C, lane % C), scale_at = 2 * S::CODES + lane * S::SROW;
+    auto issue = [&](bool any, uint32_t row, uint32_t stage) {
+        if (any) {
+            const uint32_t at = ring_at + stage;
 #pragma unroll
             for (int it = 0; it < C; it++) {
-                const int r = it * PER + lane / C, c = lane % C;
-                const int pg = __shfl_sync(0xffffffffu, page, r);
-                const size_t row = (((size_t)max(pg, 0) * p.heads + head) << p.page_shift) + ((key0 + r) & slot_mask);
-                const size_t from = row * S::ROW + 16 * c;
-                const uint32_t to = at + piece<D>(r, c);
-                copy_async<16>(to, p.k_codes + from, pg >= 0);
-                copy_async<16>(to + S::CODES, p.v_codes + from, pg >= 0);
+                const uint32_t r = __shfl_sync(0xffffffffu, row, it * PER + lane / C);
+                const bool valid = r != NONE;
+                const size_t from = valid ? (size_t)r * S::ROW : 0;
+                const uint32_t to = at + (D == 256 && (it & 1) ? piece_at ^ 64 : piece_at) + it * PER * S::ROW;
+                copy_async<16>(to, k_from + from, valid);
+                copy_async<16>(to + S::CODES, v_from + from, valid);
             }
-            const size_t row = (((size_t)max(page, 0) * p.heads + head) << p.page_shift) + ((key0 + lane) & slot_mask);
-            const uint32_t to = at + 2 * S::CODES + lane * S::SROW;
-            copy_async<S::SROW>(to, p.k_scales + row * S::SROW, page >= 0);
-            copy_async<S::SROW>(to + S::SCALES, p.v_scales + row * S::SROW, page >= 0);
+            const bool valid = row != NONE;
+            const size_t from = valid ? (size_t)row * S::SROW : 0;
+            copy_async<S::SROW>(at + scale_at, p.k_scales + from, valid);
+            copy_async<S::SROW>(at + scale_at + S::SCALES, p.v_scales + from, valid);
         }
         asm volatile("cp.async.commit_group;");
     };
-    int page_next[S::STAGES];
+    uint32_t ahead[S::STAGES];
 #pragma unroll
-    for (int i = 0; i < S::STAGES; i++) page_next[i] = page_of(i);
+    for (int i = 0; i < S::STAGES; i++) ahead[i] = row_of(i);
 #pragma unroll
-    for (int i = 0; i < S::STAGES - 1; i++) issue(i, page_next[i]);
-    int page_ahead = page_next[S::STAGES - 1];
+    for (int i = 0; i < S::STAGES - 1; i++) issue(i < tiles, ahead[i], i * S::STAGE);
+    uint32_t row_ahead = ahead[S::STAGES - 1];
 
     // q as A fragments in shared memory: [step][lane][4], rows 0-7 / 8-15 = hi / lo halves of 8 rows, or (WIDE) 16 rows,
     // hi fragments first, then lo
@@ -197,7 +220,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
         if (amax == 0.f || e > 127) e = 0;
         e = min(max(e, -126), 126);
         const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
-        if (lane == 0) col_scale[c] = scale_log2 * p.k_unit * up;
+        if (lane == 0) col_scale[c] = scale_log2 * 16.f * p.k_unit * up;   // K comes as value / 16
         __half* frag = reinterpret_cast<__half*>(smem);
 #pragma unroll
         for (int i = 0; i < N; i++) {
@@ -224,87 +247,107 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 #pragma unroll
     for (int r = 0; r < R; r++) { m[r] = -INFINITY; l[r] = 0.f; cs[r] = col_scale[g + 8 * r]; }
     const uint4* q_frag = reinterpret_cast<const uint4*>(smem) + lane;
-    const __half2 inv16 = __float2half2_rn(0.0625f), neg72 = __float2half2_rn(-72.f);
+
+    // this thread's pieces of a stage: K rows n * 8 + g (channels t D/4 ...), V rows 16 kb + 2t + {0, 1, 8, 9} (channels
+    // g D/8 ...); rows 8 apart have the same permutation
+    const int k_at = D == 64 ? piece<D>(g, t >> 1) + (t & 1) * 8 : piece<D>(g, t * (D / 128));
+    const int k_at2 = D == 256 ? piece<D>(g, 2 * t + 1) : 0;
+    const int v_piece = D == 64 ? g >> 2 : D == 128 ? g >> 1 : g, v_in = D == 64 ? (g & 3) * 4 : D == 128 ? (g & 1) * 8 : 0;
+    const int v_at[2] = {S::CODES + piece<D>(2 * t, v_piece) + v_in, S::CODES + piece<D>(2 * t + 1, v_piece) + v_in};
+    const int ks_at = 2 * S::CODES + g * S::SROW + t * (D / 64);
+    constexpr int VG = D == 256 ? 2 : 1;   // groups of a thread's channels of V
+    const int vs_at = 2 * S::CODES + S::SCALES + 2 * t * S::SROW + (D == 64 ? g >> 1 : g * VG);
+    int stage = 0, stage_in = (S::STAGES - 1) * S::STAGE;
 
     for (int i = 0; i < tiles; i++) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2));
         __syncwarp();   // the tile is there for all lanes, and the stage before it is free
-        issue(i + S::STAGES - 1, page_ahead);
-        page_ahead = page_of(i + S::STAGES);
-        const uint8_t* st = ring + (i % S::STAGES) * S::STAGE;
+        issue(i + S::STAGES - 1 < tiles, row_ahead, stage_in);
+        row_ahead = row_of(i + S::STAGES);
+        const uint8_t* st = ring + stage;
+        stage = stage == (S::STAGES - 1) * S::STAGE ? 0 : stage + S::STAGE;
+        stage_in = stage_in == (S::STAGES - 1) * S::STAGE ? 0 : stage_in + S::STAGE;
         const int key0 = begin + TILE * (warp + WARPS * i);
 
-        // ---- S = Q K^T, 8 keys at a time
+        // ---- S = Q K^T, 32 keys (4 column tiles) for each of q's fragments
+        uint32_t kw[4][D / 32];
         float a[4][4];
 #pragma unroll
         for (int n = 0; n < 4; n++) {
-            const int r = n * 8 + g;
-            uint32_t w[D / 32];
+            const uint8_t* at = st + k_at + n * 8 * S::ROW;
             if constexpr (D == 64) {
-                const uint2 v = *reinterpret_cast<const uint2*>(st + piece<D>(r, t >> 1) + (t & 1) * 8);
-                w[0] = v.x; w[1] = v.y;
+                const uint2 v = *reinterpret_cast<const uint2*>(at);
+                kw[n][0] = v.x; kw[n][1] = v.y;
             } else {
-#pragma unroll
-                for (int c = 0; c < D / 128; c++) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(st + piece<D>(r, t * (D / 128) + c));
-                    w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
+                const uint4 v = *reinterpret_cast<const uint4*>(at);
+                kw[n][0] = v.x; kw[n][1] = v.y; kw[n][2] = v.z; kw[n][3] = v.w;
+                if constexpr (D == 256) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(st + k_at2 + n * 8 * S::ROW);
+                    kw[n][4] = u.x; kw[n][5] = u.y; kw[n][6] = u.z; kw[n][7] = u.w;
                 }
             }
-            const uint8_t* sc = st + 2 * S::CODES + r * S::SROW + t * (D / 64);
-            uint32_t sw[D == 256 ? 2 : 1];   // pairs of scales
-            if constexpr (D == 64) sw[0] = *sc;
-            else if constexpr (D == 128) sw[0] = *reinterpret_cast<const uint16_t*>(sc);
-            else { const uint32_t v = *reinterpret_cast<const uint32_t*>(sc); sw[0] = v & 0xffff; sw[1] = v >> 16; }
 #pragma unroll
-            for (int r4 = 0; r4 < 4; r4++) a[n][r4] = 0.f;
+            for (int x = 0; x < 4; x++) a[n][x] = 0.f;
+        }
 #pragma unroll
-            for (int wi = 0; wi < D / 32; wi++) {
-                const __half2 two = as_half2(kv_scales_to_half(sw[wi / 4]));
-                const __half2 one = (wi / 2) & 1 ? __high2half2(two) : __low2half2(two);
-                uint32_t h[4];
-                dequantise(w[wi], __hmul2(one, inv16), __hmul2(one, neg72), h);
+        for (int gr = 0; gr < D / 64; gr++) {      // groups of this thread's channels, two words each
+            Scale sc[4];
+#pragma unroll
+            for (int n = 0; n < 4; n++) sc[n] = scale_of(kv_scales_to_half((uint32_t)st[ks_at + n * 8 * S::SROW + gr] * 0x101u));
+#pragma unroll
+            for (int wi = 2 * gr; wi < 2 * gr + 2; wi++) {
+                uint4 f[2], f2[2];
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const uint4 f = q_frag[(2 * wi + u) * 32];
-                    const uint32_t qa[4] = {f.x, f.y, f.z, f.w};
-                    mma(a[n], qa, h[2 * u], h[2 * u + 1]);
-                    if (WIDE) {
-                        const uint4 f2 = q_frag[(S::STEPS + 2 * wi + u) * 32];
-                        const uint32_t ql[4] = {f2.x, f2.y, f2.z, f2.w};
-                        mma(a[n], ql, h[2 * u], h[2 * u + 1]);
+                    f[u] = q_frag[(2 * wi + u) * 32];
+                    if (WIDE) f2[u] = q_frag[(S::STEPS + 2 * wi + u) * 32];
+                }
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    uint32_t h[4];
+                    dequantise(kw[n][wi], sc[n], masks, h);
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const uint32_t qa[4] = {f[u].x, f[u].y, f[u].z, f[u].w};
+                        mma(a[n], qa, h[2 * u], h[2 * u + 1]);
+                        if (WIDE) {
+                            const uint32_t ql[4] = {f2[u].x, f2[u].y, f2[u].z, f2[u].w};
+                            mma(a[n], ql, h[2 * u], h[2 * u + 1]);
+                        }
                     }
                 }
             }
         }
 
-        // ---- V's scales: bytes of keys 2t, 2t + 1, 2t + 8, 2t + 9 of each 16-key half, this thread's channel groups
-        constexpr int VG = D == 256 ? 2 : 1;
-        uint32_t vs[2][VG];
+        // ---- V's scales: pairs (key 2t, 2t + 1) and (2t + 8, 2t + 9) of each 16-key half
+        uint32_t vs[2][2][VG];
         uint32_t nan = 0;
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
-            const uint8_t* sc = st + 2 * S::CODES + S::SCALES + (16 * kb + 2 * t) * S::SROW + (D == 64 ? g >> 1 : g * VG);
+        for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-            for (int x = 0; x < VG; x++) {
-                vs[kb][x] = (uint32_t)sc[x] | (uint32_t)sc[S::SROW + x] << 8 | (uint32_t)sc[8 * S::SROW + x] << 16 |
-                            (uint32_t)sc[9 * S::SROW + x] << 24;
-                nan |= (vs[kb][x] + 0x01010101u) & 0x80808080u;
-            }
-        }
+            for (int y = 0; y < 2; y++)
+#pragma unroll
+                for (int x = 0; x < VG; x++) {
+                    const uint8_t* sc = st + vs_at + (16 * kb + 8 * y) * S::SROW + x;
+                    vs[kb][y][x] = (uint32_t)sc[0] + (uint32_t)sc[S::SROW] * 256u;
+                    nan |= vs[kb][y][x] + 0x0101u;
+                }
         // A NaN in a value must not meet the zero weights of rows that do not see it: its scale becomes 0 and the
         // weights of the rows that see it become NaN.
         uint32_t poison = 0;   // keys of the tile
-        if (__any_sync(0xffffffffu, nan)) {
+        if (__any_sync(0xffffffffu, nan & 0x8080u)) {
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-                for (int x = 0; x < VG; x++)
+                for (int y = 0; y < 2; y++)
 #pragma unroll
-                    for (int y = 0; y < 4; y++)
-                        if ((vs[kb][x] >> (8 * y) & 0x7f) == 0x7f) {
-                            vs[kb][x] &= ~(0xffu << (8 * y));
-                            poison |= 1u << (16 * kb + 2 * t + (y & 1) + (y >> 1) * 8);
-                        }
+                    for (int x = 0; x < VG; x++)
+#pragma unroll
+                        for (int z = 0; z < 2; z++)
+                            if ((vs[kb][y][x] >> (8 * z) & 0x7f) == 0x7f) {
+                                vs[kb][y][x] &= ~(0xffu << (8 * z));
+                                poison |= 1u << (16 * kb + 8 * y + 2 * t + z);
+                            }
             poison = __reduce_or_sync(0xffffffffu, poison);
         }
 
@@ -374,18 +417,17 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
         // ---- O += P V, 16 keys at a time
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
-            const uint8_t* vt = st + S::CODES;
             uint32_t w[4][D / 64];   // keys 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
             for (int y = 0; y < 4; y++) {
-                const int r = 16 * kb + 2 * t + (y & 1) + (y >> 1) * 8;
+                const uint8_t* at = st + v_at[y & 1] + (16 * kb + (y >> 1) * 8) * S::ROW;
                 if constexpr (D == 64) {
-                    w[y][0] = *reinterpret_cast<const uint32_t*>(vt + piece<D>(r, g >> 2) + (g & 3) * 4);
+                    w[y][0] = *reinterpret_cast<const uint32_t*>(at);
                 } else if constexpr (D == 128) {
-                    const uint2 v = *reinterpret_cast<const uint2*>(vt + piece<D>(r, g >> 1) + (g & 1) * 8);
+                    const uint2 v = *reinterpret_cast<const uint2*>(at);
                     w[y][0] = v.x; w[y][1] = v.y;
                 } else {
-                    const uint4 v = *reinterpret_cast<const uint4*>(vt + piece<D>(r, g));
+                    const uint4 v = *reinterpret_cast<const uint4*>(at);
                     w[y][0] = v.x; w[y][1] = v.y; w[y][2] = v.z; w[y][3] = v.w;
                 }
             }
@@ -394,15 +436,14 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
             const uint32_t pl[4] = {lo[0][2 * kb], lo[R - 1][2 * kb], lo[0][2 * kb + 1], lo[R - 1][2 * kb + 1]};
 #pragma unroll
             for (int wi = 0; wi < D / 64; wi++) {
-                const uint32_t sc = vs[kb][wi / 2 % VG];
-                const __half2 sa = as_half2(kv_scales_to_half(sc & 0xffff)), sb = as_half2(kv_scales_to_half(sc >> 16));
-                const __half2 a16 = __hmul2(sa, inv16), a72 = __hmul2(sa, neg72), b16 = __hmul2(sb, inv16), b72 = __hmul2(sb, neg72);
+                const Scale sa = scale_of(kv_scales_to_half(vs[kb][0][wi / 2 % VG]));
+                const Scale sb = scale_of(kv_scales_to_half(vs[kb][1][wi / 2 % VG]));
 #pragma unroll
                 for (int half = 0; half < 2; half++) {   // channels 0-3, 4-7 of the words
                     const uint32_t sel = half ? 0x7632 : 0x5410;
                     uint32_t h0[4], h1[4];
-                    dequantise(__byte_perm(w[0][wi], w[1][wi], sel), a16, a72, h0);
-                    dequantise(__byte_perm(w[2][wi], w[3][wi], sel), b16, b72, h1);
+                    dequantise(__byte_perm(w[0][wi], w[1][wi], sel), sa, masks, h0);
+                    dequantise(__byte_perm(w[2][wi], w[3][wi], sel), sb, masks, h1);
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         mma(o[8 * wi + 4 * half + j], pa, h0[j], h1[j]);
@@ -451,7 +492,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
         }
         const size_t row = (size_t)(first + ci / group) * hq + head * group + ci % group;
         if (parts == 1) {
-            const float inv = L == 0.f ? 0.f : p.v_unit / L;
+            const float inv = L == 0.f ? 0.f : 16.f * p.v_unit / L;   // V comes as value / 16
             float* dst = out + row * D + d;
             dst[0] = acc.x * inv; dst[1] = acc.y * inv; dst[2] = acc.z * inv; dst[3] = acc.w * inv;
         } else {
@@ -467,7 +508,7 @@ template <int D>
 __global__ void __launch_bounds__(THREADS) k_attn_paged_join(float* __restrict__ out, int hq, KvBatchDev b, float v_unit, Split sp,
                                                              const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
     constexpr int N = D / 32;
-    __shared__ float sm_l[WARPS], sm_m[WARPS];
+    __shared__ float sm_l[WARPS];
     __shared__ float sm_o[WARPS][D];
     const int s = blockIdx.z, i = blockIdx.y, h = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int first, count;
@@ -476,37 +517,46 @@ __global__ void __launch_bounds__(THREADS) k_attn_paged_join(float* __restrict__
     asm volatile("griddepcontrol.wait;" ::: "memory");   // also before an early return: the next kernel waits for this one only
     if (i >= count || parts <= 1) return;
     const size_t row = (size_t)(first + i) * hq + h;
-    float m = -INFINITY, l = 0.f, o[N];
+    const float2* ml = part_ml + row * sp.splits;
+    const float* po = part_o + row * sp.splits * D + lane;
+    float M = -INFINITY;   // every warp finds the maximum by itself
+    for (int c = lane; c < parts; c += 32) M = fmaxf(M, ml[c].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float l = 0.f, o[N];
 #pragma unroll
     for (int n = 0; n < N; n++) o[n] = 0.f;
-    for (int c = warp; c < parts; c += WARPS) {
-        const float2 ml = part_ml[row * sp.splits + c];
-        const float* po = part_o + (row * sp.splits + c) * D + lane;
-        const float mx = fmaxf(m, ml.x);
-        const float old = m == -INFINITY ? 1.f : ex2(m - mx), f = ml.x == -INFINITY ? 1.f : ex2(ml.x - mx);
-        l = l * old + ml.y * f;
+    // warp w takes chunks w, w + 4, ...: 32 of their weights at a time, one per lane
+    for (int c0 = warp; c0 < parts; c0 += 32 * WARPS) {
+        const int c = c0 + lane * WARPS;
+        float f = 0.f;
+        if (c < parts) {
+            const float2 v = ml[c];
+            f = v.x == -INFINITY ? 1.f : ex2(v.x - M);   // a chunk without a visible key holds zeros (or NaN)
+            l += f * v.y;
+        }
+        const int n_here = min(32, (parts - c0 + WARPS - 1) / WARPS);
+#pragma unroll 4
+        for (int x = 0; x < n_here; x++) {
+            const float fx = __shfl_sync(0xffffffffu, f, x);
 #pragma unroll
-        for (int n = 0; n < N; n++) o[n] = o[n] * old + po[32 * n] * f;
-        m = mx;
+            for (int n = 0; n < N; n++) o[n] = fmaf(fx, po[(size_t)(c0 + x * WARPS) * D + 32 * n], o[n]);
+        }
     }
-    if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+    if (lane == 0) sm_l[warp] = l;
 #pragma unroll
     for (int n = 0; n < N; n++) sm_o[warp][lane + 32 * n] = o[n];
     __syncthreads();
-    float M = -INFINITY, L = 0.f;
+    float L = 0.f;
 #pragma unroll
-    for (int w = 0; w < WARPS; w++) M = fmaxf(M, sm_m[w]);
-    float f[WARPS];
-#pragma unroll
-    for (int w = 0; w < WARPS; w++) {
-        f[w] = sm_m[w] == -INFINITY ? 1.f : ex2(sm_m[w] - M);
-        L += f[w] * sm_l[w];
-    }
-    const float inv = L == 0.f ? 0.f : v_unit / L;
+    for (int w = 0; w < WARPS; w++) L += sm_l[w];
+    const float inv = L == 0.f ? 0.f : 16.f * v_unit / L;
     for (int d = threadIdx.x; d < D; d += THREADS) {
         float acc = 0.f;
 #pragma unroll
-        for (int w = 0; w < WARPS; w++) acc += f[w] * sm_o[w][d];
+        for (int w = 0; w < WARPS; w++) acc += sm_o[w][d];
         out[row * D + d] = acc * inv;
     }
 }

@@ -159,6 +159,7 @@ lancius_error lcu_kv_describe(const lcu_kv_pages* pages, const lcu_kv_batch* bat
     if (batch->n_seqs > 65535 || batch->n_tokens > (size_t)INT32_MAX / 2 || batch->table_width > (size_t)INT32_MAX / ps)
         return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
     if (!batch->token_start && batch->n_tokens < batch->n_seqs) return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
+    if (pages->n_pages > 0xfffffffeull / ps / pages->n_heads) return bad(LANCIUS_ERROR_SHAPE_MISMATCH);   // 32-bit row numbers
     const size_t whole = batch->table_width * ps;
     p->k_codes = pages->k_codes; p->v_codes = pages->v_codes;
     p->k_scales = pages->k_scales; p->v_scales = pages->v_scales;
