@@ -7,20 +7,21 @@
 // ((new token, query head) pairs, up to 8 or 16 per CTA); at the measured copy rate an SM receives about 46
 // codes a clock, so turning codes into operands is the work that has to fit beside the loads.
 //
-// Products run as mma.sync m16n8k16 (f16 in, FP32 out). Measured 0.5 of them per clock and SM, each covers 128
-// codes: 64 codes a clock, above the HBM rate. tcgen05 would need the operands written to shared or tensor
+// Products run as mma.sync m16n8k16 (f16 in, FP32 out). Measured 0.5 of them per clock and SM; two serve 256 codes
+// and 8 rows, so 64 codes a clock, above the HBM rate. tcgen05 would need the operands written to shared or tensor
 // memory as f16 first, four times the bytes of the codes. The operands are exact: a dequantised value
 // (n - 8) * scale has 8 significant bits, so K and V fit f16 as they are; q (scaled to [1, 2) by a power of two) and p are
-// split into two f16 halves, 22 bits. With at most 8 rows the halves are the two row halves of one MMA (rows
-// 0-7 hi, 8-15 lo, added afterwards); with 9 to 16 rows (WIDE) they are two MMAs.
+// split into two f16 halves, 22 bits, one MMA each. The codes are operand A (16 keys or 16 channels), q and p operand B (8
+// rows): of the two assignments the one whose accumulator for O is half as large, which decides how many warps
+// fit (measured with q and p as A, halves stacked in its 16 rows: 160 registers, 63.4 us at 131072 keys x 8 heads x 128).
 //
 // Dequantising: a code or'ed into the mantissa of an f16 constant, then one HFMA2 with the group's factor and offset
 // gives (n - 8) scale / 16 without rounding (scale_of). Eight codes take 5 integer and 4 HFMA2 instructions. (4-bit
 // floating point needs cvt, measured 25 codes a clock and SM, or more shifts.)
-//   S = Q K^T: B operand = K^T, whose fragment wants channel pairs of one key: a thread holds D / 4 contiguous
-//     channels of a key, any order of channels will do if q's fragment has the same.
-//   O += P V: B operand = V, whose fragment wants key pairs of one channel: the words of two keys are first
-//     interleaved by 16-bit halves (2 PRMT per 16 codes). S's accumulator layout is P's operand layout.
+//   S^T = K Q^T: A = K wants channel pairs of one key: a thread holds D / 4 contiguous channels of a key, any order of
+//     channels will do if q's fragment has the same.
+//   O^T += V^T P^T: A = V^T wants key pairs of one channel: the words of two keys are first interleaved by 16-bit
+//     halves (2 PRMT per 16 codes). P^T comes from S^T's accumulators by movmatrix.
 //
 // Work: CTA = (chunk of keys, key head, sequence, block of rows), 4 warps that each take every fourth tile of 32
 // keys through a ring of cp.async stages of their own (no block barrier in the loop) and are merged at the end.
@@ -43,17 +44,17 @@ __device__ int g_attn_paged_fault = 0;
 template <int D, bool WIDE>
 struct Shape {
     static constexpr int ROW = D / 2, SROW = D / 16;            // code and scale bytes of a cached row
-    static constexpr int STAGES = D == 256 ? 2 : D == 128 ? 3 : 4;
+    static constexpr int STAGES = D == 256 ? 2 : D == 128 ? (WIDE ? 3 : 2) : 4;
     static constexpr int CODES = TILE * ROW, SCALES = TILE * SROW;
     static constexpr int STAGE = 2 * (CODES + SCALES);
-    static constexpr int COLS = WIDE ? 16 : 8;                  // rows of q that one CTA serves
+    static constexpr int NT = WIDE ? 2 : 1, COLS = 8 * NT;      // rows of q that one CTA serves
     static constexpr int STEPS = D / 16;
-    static constexpr int Q_BYTES = STEPS * 512 * (WIDE ? 2 : 1);
+    static constexpr int Q_BYTES = STEPS * 512 * NT;
     static constexpr int RING = WARPS * STAGES * STAGE;
     static constexpr int O_LD = D + 4;
     static constexpr int MERGE = WARPS * COLS * O_LD * 4;       // reuses the ring
     static constexpr int SMEM = Q_BYTES + (RING > MERGE ? RING : MERGE);
-    static constexpr int RESIDENT = D == 256 ? 2 : D == 128 ? 3 : WIDE ? 4 : 5;   // CTAs per SM that registers and SMEM allow
+    static constexpr int RESIDENT = D == 256 ? 2 : D == 128 ? (WIDE ? 3 : 4) : WIDE ? 4 : 5;   // CTAs per SM
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -110,6 +111,11 @@ __device__ __forceinline__ int piece(int r, int c) {
     return r * 128 + ((c ^ ((((r >> 1) & 3) << 1) | (r & 1))) << 4);
 }
 
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {   // of an 8 x 8 f16 matrix held by the warp
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
 // split of p0, p1 into f16 halves
 __device__ __forceinline__ void split(float p0, float p1, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(p0, p1);
@@ -125,7 +131,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D, WIDE>::RESIDENT)
 k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, int hq, KvPagesDev p, KvBatchDev b,
              float scale_log2, Split sp, float* __restrict__ part_o, float2* __restrict__ part_ml) {
     using S = Shape<D, WIDE>;
-    constexpr int COLS = S::COLS, R = WIDE ? 2 : 1;   // rows of q per thread
+    constexpr int COLS = S::COLS, NT = S::NT, R = 2 * NT;   // R rows of q per thread: 2t, 2t + 1 (and 8 more)
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float col_scale[COLS];
     __shared__ float sm_m[WARPS][COLS], sm_l[WARPS][COLS];
@@ -153,7 +159,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     };
     int limit[R], least = 0x7fffffff;
 #pragma unroll
-    for (int r = 0; r < R; r++) limit[r] = limit_of(g + 8 * r);
+    for (int r = 0; r < R; r++) limit[r] = limit_of(2 * t + (r & 1) + (r >> 1) * 8);
     least = limit_of(0);                                          // positions rise with the row
     const int begin = split_id * sp.chunk, end = min(begin + sp.chunk, limit_of(cols - 1));
 
@@ -203,8 +209,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     for (int i = 0; i < S::STAGES - 1; i++) issue(i < tiles, ahead[i], i * S::STAGE);
     uint32_t row_ahead = ahead[S::STAGES - 1];
 
-    // q as A fragments in shared memory: [step][lane][4], rows 0-7 / 8-15 = hi / lo halves of 8 rows, or (WIDE) 16 rows,
-    // hi fragments first, then lo
+    // q as B fragments in shared memory: [8 rows][step][lane][hi 0, hi 1, lo 0, lo 1]
     for (int c = warp; c < COLS; c += WARPS) {
         constexpr int N = D / 32;
         const int ci = block * COLS + c;
@@ -227,25 +232,22 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
             const int ch = lane + 32 * i, owner = ch / (D / 4), in = ch % (D / 4), step = in / 8 * 2 + ((in & 3) >> 1);
             const float y = x[i] * down;
             const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
-            const int at = ((step * 32 + (c & 7) * 4 + owner) * 4 + (in & 1) * 2) * 2 + ((in >> 2) & 1);   // register 0 or 2
-            if (WIDE) {
-                frag[at + (c >> 3) * 2] = hi;
-                frag[at + (c >> 3) * 2 + S::STEPS * 256] = lo;
-            } else {
-                frag[at] = hi;
-                frag[at + 2] = lo;
-            }
+            const int at = ((((c >> 3) * S::STEPS + step) * 32 + (c & 7) * 4 + owner) * 4 + (in & 1)) * 2 + ((in >> 2) & 1);
+            frag[at] = hi;
+            frag[at + 4] = lo;
         }
     }
     __syncthreads();
 
-    float o[D / 8][4], m[R], l[R], cs[R];
+    float o[NT][D / 16][4], m[R], l[R], cs[R];   // o: channels g D/8 + 2j, + 2j + 1 of rows 2t, 2t + 1
 #pragma unroll
-    for (int j = 0; j < D / 8; j++)
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) o[j][r] = 0.f;
+        for (int j = 0; j < D / 16; j++)
 #pragma unroll
-    for (int r = 0; r < R; r++) { m[r] = -INFINITY; l[r] = 0.f; cs[r] = col_scale[g + 8 * r]; }
+            for (int r = 0; r < 4; r++) o[nt][j][r] = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; r++) { m[r] = -INFINITY; l[r] = 0.f; cs[r] = col_scale[2 * t + (r & 1) + (r >> 1) * 8]; }
     const uint4* q_frag = reinterpret_cast<const uint4*>(smem) + lane;
 
     // this thread's pieces of a stage: K rows n * 8 + g (channels t D/4 ...), V rows 16 kb + 2t + {0, 1, 8, 9} (channels
@@ -269,9 +271,9 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
         stage_in = stage_in == (S::STAGES - 1) * S::STAGE ? 0 : stage_in + S::STAGE;
         const int key0 = begin + TILE * (warp + WARPS * i);
 
-        // ---- S = Q K^T, 32 keys (4 column tiles) for each of q's fragments
+        // ---- S^T = K Q^T, 32 keys for each of q's fragments
         uint32_t kw[4][D / 32];
-        float a[4][4];
+        float a[NT][2][4];   // [.][16 keys]: (key g, rows 2t, 2t + 1), (key g + 8, the same)
 #pragma unroll
         for (int n = 0; n < 4; n++) {
             const uint8_t* at = st + k_at + n * 8 * S::ROW;
@@ -286,9 +288,11 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
                     kw[n][4] = u.x; kw[n][5] = u.y; kw[n][6] = u.z; kw[n][7] = u.w;
                 }
             }
-#pragma unroll
-            for (int x = 0; x < 4; x++) a[n][x] = 0.f;
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int x = 0; x < 8; x++) a[nt][x >> 2][x & 3] = 0.f;
 #pragma unroll
         for (int gr = 0; gr < D / 64; gr++) {      // groups of this thread's channels, two words each
             Scale sc[4];
@@ -296,23 +300,23 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
             for (int n = 0; n < 4; n++) sc[n] = scale_of(kv_scales_to_half((uint32_t)st[ks_at + n * 8 * S::SROW + gr] * 0x101u));
 #pragma unroll
             for (int wi = 2 * gr; wi < 2 * gr + 2; wi++) {
-                uint4 f[2], f2[2];
+                uint4 f[NT][2];
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    f[u] = q_frag[(2 * wi + u) * 32];
-                    if (WIDE) f2[u] = q_frag[(S::STEPS + 2 * wi + u) * 32];
-                }
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    uint32_t h[4];
-                    dequantise(kw[n][wi], sc[n], masks, h);
+                    for (int u = 0; u < 2; u++) f[nt][u] = q_frag[(nt * S::STEPS + 2 * wi + u) * 32];
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++) {
+                    uint32_t h[4], h8[4];
+                    dequantise(kw[2 * kb][wi], sc[2 * kb], masks, h);
+                    dequantise(kw[2 * kb + 1][wi], sc[2 * kb + 1], masks, h8);
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
-                        const uint32_t qa[4] = {f[u].x, f[u].y, f[u].z, f[u].w};
-                        mma(a[n], qa, h[2 * u], h[2 * u + 1]);
-                        if (WIDE) {
-                            const uint32_t ql[4] = {f2[u].x, f2[u].y, f2[u].z, f2[u].w};
-                            mma(a[n], ql, h[2 * u], h[2 * u + 1]);
+                        const uint32_t ka[4] = {h[2 * u], h8[2 * u], h[2 * u + 1], h8[2 * u + 1]};
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            mma(a[nt][kb], ka, f[nt][u].x, f[nt][u].y);
+                            mma(a[nt][kb], ka, f[nt][u].z, f[nt][u].w);
                         }
                     }
                 }
@@ -351,70 +355,67 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
             poison = __reduce_or_sync(0xffffffffu, poison);
         }
 
-        // ---- weights
-        float sv[R][8], top[R];
+        // ---- weights. Value x of a row: key key0 + 16 (x >> 1) + 8 (x & 1) + g
+        float sv[R][4], top[R];
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-            top[r] = -INFINITY;
+        for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int n = 0; n < 4; n++)
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    float x = WIDE ? a[n][2 * r + u] : a[n][u] + a[n][2 + u];
-                    x *= cs[r];
-                    sv[r][2 * n + u] = x;
-                }
-        }
+            for (int x = 0; x < 4; x++) sv[r][x] = a[r >> 1][x >> 1][2 * (x & 1) + (r & 1)] * cs[r];
         if (key0 + TILE > least) {
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int x = 0; x < 8; x++)
-                    if (key0 + (x >> 1) * 8 + 2 * t + (x & 1) >= limit[r]) sv[r][x] = -INFINITY;
+                for (int x = 0; x < 4; x++)
+                    if (key0 + 8 * x + g >= limit[r]) sv[r][x] = -INFINITY;
         }
         bool raise = false;
 #pragma unroll
         for (int r = 0; r < R; r++) {
-#pragma unroll
-            for (int x = 0; x < 8; x++) top[r] = fmaxf(top[r], sv[r][x]);
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+            top[r] = fmaxf(fmaxf(sv[r][0], sv[r][1]), fmaxf(sv[r][2], sv[r][3]));
             raise = raise || top[r] > m[r] + RAISE;
         }
-        if (__any_sync(0xffffffffu, raise)) {
+        if (__any_sync(0xffffffffu, raise)) {   // some key exceeds its row's maximum by enough
             float f[R];
 #pragma unroll
             for (int r = 0; r < R; r++) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], x));
                 const float mx = fmaxf(m[r], top[r]);
                 f[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - mx);   // nothing was summed before the first key
                 m[r] = mx;
                 l[r] *= f[r];
             }
 #pragma unroll
-            for (int j = 0; j < D / 8; j++) {
-                o[j][0] *= f[0]; o[j][1] *= f[0];
-                o[j][2] *= f[R - 1]; o[j][3] *= f[R - 1];
-            }
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int j = 0; j < D / 16; j++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) o[nt][j][x] *= f[2 * nt + (x & 1)];
         }
-        uint32_t hi[R][4], lo[R][4];
+        uint32_t hi[NT][4], lo[NT][4];   // P^T fragments of keys 8 x ...
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-            const float base = m[r] == -INFINITY ? 0.f : m[r] - P_BIAS;
-            float pw[8];
+        for (int nt = 0; nt < NT; nt++) {
+            float pw[2][4];
 #pragma unroll
-            for (int x = 0; x < 8; x++) {
-                pw[x] = ex2(sv[r][x] - base);
-                if (poison) {
-                    const int k = (x >> 1) * 8 + 2 * t + (x & 1);
-                    if ((poison >> k & 1) && key0 + k < limit[r]) pw[x] = NAN;
+            for (int u = 0; u < 2; u++) {
+                const int r = 2 * nt + u;
+                const float base = m[r] == -INFINITY ? 0.f : m[r] - P_BIAS;
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    pw[u][x] = ex2(sv[r][x] - base);
+                    if (poison && (poison >> (8 * x + g) & 1) && key0 + 8 * x + g < limit[r]) pw[u][x] = NAN;
+                    l[r] += pw[u][x];
                 }
-                l[r] += pw[x];
             }
 #pragma unroll
-            for (int n = 0; n < 4; n++) split(pw[2 * n], pw[2 * n + 1], hi[r][n], lo[r][n]);
+            for (int x = 0; x < 4; x++) {
+                split(pw[0][x], pw[1][x], hi[nt][x], lo[nt][x]);
+                hi[nt][x] = transpose8(hi[nt][x]);
+                lo[nt][x] = transpose8(lo[nt][x]);
+            }
         }
 
-        // ---- O += P V, 16 keys at a time
+        // ---- O^T += V^T P^T, 16 keys at a time
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
             uint32_t w[4][D / 64];   // keys 2t, 2t + 1, 2t + 8, 2t + 9
@@ -431,9 +432,6 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
                     w[y][0] = v.x; w[y][1] = v.y; w[y][2] = v.z; w[y][3] = v.w;
                 }
             }
-            const uint32_t pa[4] = {hi[0][2 * kb], WIDE ? hi[R - 1][2 * kb] : lo[0][2 * kb], hi[0][2 * kb + 1],
-                                    WIDE ? hi[R - 1][2 * kb + 1] : lo[0][2 * kb + 1]};
-            const uint32_t pl[4] = {lo[0][2 * kb], lo[R - 1][2 * kb], lo[0][2 * kb + 1], lo[R - 1][2 * kb + 1]};
 #pragma unroll
             for (int wi = 0; wi < D / 64; wi++) {
                 const Scale sa = scale_of(kv_scales_to_half(vs[kb][0][wi / 2 % VG]));
@@ -445,9 +443,13 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
                     dequantise(__byte_perm(w[0][wi], w[1][wi], sel), sa, masks, h0);
                     dequantise(__byte_perm(w[2][wi], w[3][wi], sel), sb, masks, h1);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        mma(o[8 * wi + 4 * half + j], pa, h0[j], h1[j]);
-                        if (WIDE) mma(o[8 * wi + 4 * half + j], pl, h0[j], h1[j]);
+                    for (int j = 0; j < 2; j++) {   // channels 2j, 2j + 1 of the four
+                        const uint32_t va[4] = {h0[2 * j], h0[2 * j + 1], h1[2 * j], h1[2 * j + 1]};
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            mma(o[nt][4 * wi + 2 * half + j], va, hi[nt][2 * kb], hi[nt][2 * kb + 1]);
+                            mma(o[nt][4 * wi + 2 * half + j], va, lo[nt][2 * kb], lo[nt][2 * kb + 1]);
+                        }
                     }
                 }
             }
@@ -455,25 +457,23 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     }
     asm volatile("cp.async.wait_all;");
 
-    // ---- merge the warps. Thread (g, t) holds channels 2t D/8 + j and (2t + 1) D/8 + j of its rows.
+    // ---- merge the warps
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        if (t == 0) { sm_m[warp][g + 8 * r] = m[r]; sm_l[warp][g + 8 * r] = l[r]; }
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
+        const int c = 2 * t + (r & 1) + (r >> 1) * 8;
+        if (g == 0) { sm_m[warp][c] = m[r]; sm_l[warp][c] = l[r]; }
     }
     __syncthreads();   // every ring is idle
     float* so = reinterpret_cast<float*>(smem + S::Q_BYTES);
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        float* at = so + (warp * COLS + g + 8 * r) * S::O_LD + 2 * t * (D / 8);
+        float* at = so + (warp * COLS + 2 * t + (r & 1) + (r >> 1) * 8) * S::O_LD + g * (D / 8);
 #pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int j = 0; j < D / 8; j += 4) {
-                auto v = [&](int x) { return WIDE ? o[j + x][2 * r + u] : o[j + x][u] + o[j + x][2 + u]; };
-                *reinterpret_cast<float4*>(at + u * (D / 8) + j) = make_float4(v(0), v(1), v(2), v(3));
-            }
+        for (int j = 0; j < D / 16; j += 2)
+            *reinterpret_cast<float4*>(at + 2 * j) = make_float4(o[r >> 1][j][r & 1], o[r >> 1][j][2 + (r & 1)],
+                                                                 o[r >> 1][j + 1][r & 1], o[r >> 1][j + 1][2 + (r & 1)]);
     }
     __syncthreads();
     for (int x = tid; x < cols * (D / 4); x += THREADS) {
