@@ -41,20 +41,21 @@ constexpr float RAISE = 8.f;      // the running maximum moves only when exceede
 
 __device__ int g_attn_paged_fault = 0;
 
-template <int D, bool WIDE>
+template <int D, int ROWS>   // ROWS of q per CTA: 4, 8 or 16
 struct Shape {
     static constexpr int ROW = D / 2, SROW = D / 16;            // code and scale bytes of a cached row
-    static constexpr int STAGES = D == 256 ? 2 : D == 128 ? (WIDE ? 3 : 2) : 4;
+    static constexpr int STAGES = D == 256 ? 2 : D == 128 ? (ROWS == 16 ? 3 : 2) : 4;
     static constexpr int CODES = TILE * ROW, SCALES = TILE * SROW;
     static constexpr int STAGE = 2 * (CODES + SCALES);
-    static constexpr int NT = WIDE ? 2 : 1, COLS = 8 * NT;      // rows of q that one CTA serves
+    static constexpr int NT = ROWS == 16 ? 2 : 1;               // 8-column operands
+    static constexpr bool PACK = ROWS == 4;                     // hi and lo halves share one
     static constexpr int STEPS = D / 16;
-    static constexpr int Q_BYTES = STEPS * 512 * NT;
+    static constexpr int Q_BYTES = STEPS * (PACK ? 256 : 512) * NT;
     static constexpr int RING = WARPS * STAGES * STAGE;
     static constexpr int O_LD = D + 4;
-    static constexpr int MERGE = WARPS * COLS * O_LD * 4;       // reuses the ring
+    static constexpr int MERGE = WARPS * ROWS * O_LD * 4;       // reuses the ring
     static constexpr int SMEM = Q_BYTES + (RING > MERGE ? RING : MERGE);
-    static constexpr int RESIDENT = D == 256 ? 2 : D == 128 ? (WIDE ? 3 : 4) : WIDE ? 4 : 5;   // CTAs per SM
+    static constexpr int RESIDENT = D == 256 ? 2 : D == 128 ? (ROWS == 16 ? 3 : 4) : ROWS == 16 ? 4 : 5;   // CTAs per SM
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -64,20 +65,25 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 template <int N>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src));
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N));
+}
+template <int N>   // zeros when !valid
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool valid) {
     const int n = valid ? N : 0;
     if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n));
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(N));
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-// A group's scale s (in both halves of `two`) as the factors and offsets of its codes: codes in bits 0-3 of a 16-bit
+// Scales of two groups or keys (the halves of `two`) as the factors and offsets of its codes: codes in bits 0-3 of a 16-bit
 // half, or'ed with 0x6400, are the f16 number 1024 + n, those in bits 4-7 are 16 (64 + n). All are exact: s has 4
 // significant bits, 129 * 15 < 2^11. Values come out as (n - 8) s / 16, so that 64.5 s stays below f16's largest.
 struct Scale { __half2 m0, b0, m4, b4; };
@@ -85,6 +91,10 @@ __device__ __forceinline__ Scale scale_of(uint32_t two) {
     const __half2 s = as_half2(two);
     return Scale{__hmul2(s, __float2half2_rn(0.0625f)), __hmul2(s, __float2half2_rn(-64.5f)),
                  __hmul2(s, __float2half2_rn(0.00390625f)), __hmul2(s, __float2half2_rn(-4.5f))};
+}
+__device__ __forceinline__ Scale half_of(const Scale& s, int high) {
+    return high ? Scale{__high2half2(s.m0), __high2half2(s.b0), __high2half2(s.m4), __high2half2(s.b4)}
+                : Scale{__low2half2(s.m0), __low2half2(s.b0), __low2half2(s.m4), __low2half2(s.b4)};
 }
 // The masks are held in registers that the compiler cannot see through: (w & mask) | bias with two immediates would
 // take two LOP3, and these are the instructions that the kernel executes most.
@@ -126,12 +136,13 @@ __device__ __forceinline__ void split(float p0, float p1, uint32_t& hi, uint32_t
 
 struct Split { int chunk, splits; };
 
-template <int D, bool WIDE>
-__global__ void __launch_bounds__(THREADS, Shape<D, WIDE>::RESIDENT)
+template <int D, int ROWS>
+__global__ void __launch_bounds__(THREADS, Shape<D, ROWS>::RESIDENT)
 k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, int hq, KvPagesDev p, KvBatchDev b,
              float scale_log2, Split sp, float* __restrict__ part_o, float2* __restrict__ part_ml) {
-    using S = Shape<D, WIDE>;
-    constexpr int COLS = S::COLS, NT = S::NT, R = 2 * NT;   // R rows of q per thread: 2t, 2t + 1 (and 8 more)
+    using S = Shape<D, ROWS>;
+    constexpr int COLS = ROWS, NT = S::NT, R = 2 * NT;
+    constexpr bool PACK = S::PACK;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float col_scale[COLS];
     __shared__ float sm_m[WARPS][COLS], sm_l[WARPS][COLS];
@@ -152,6 +163,8 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     const int parts = max(1, (keys + sp.chunk - 1) / sp.chunk);   // chunks of this sequence
     if (cols <= 0 || split_id >= parts) return;
 
+    // this thread's R rows of q: 2t, 2t + 1 (and 8 more); packed: 2 (t % 2) and the next, held by t and t ^ 2
+    auto row_at = [&](int r) { return PACK ? 2 * (t & 1) + r : 2 * t + (r & 1) + (r >> 1) * 8; };
     // keys that row c of the block sees: those up to its token's position
     auto limit_of = [&](int c) {
         const int i = (block * COLS + c) / group;
@@ -159,7 +172,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     };
     int limit[R], least = 0x7fffffff;
 #pragma unroll
-    for (int r = 0; r < R; r++) limit[r] = limit_of(2 * t + (r & 1) + (r >> 1) * 8);
+    for (int r = 0; r < R; r++) limit[r] = limit_of(row_at(r));
     least = limit_of(0);                                          // positions rise with the row
     const int begin = split_id * sp.chunk, end = min(begin + sp.chunk, limit_of(cols - 1));
 
@@ -186,19 +199,29 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     auto issue = [&](bool any, uint32_t row, uint32_t stage) {
         if (any) {
             const uint32_t at = ring_at + stage;
+            if (__all_sync(0xffffffffu, row != NONE)) {
 #pragma unroll
-            for (int it = 0; it < C; it++) {
-                const uint32_t r = __shfl_sync(0xffffffffu, row, it * PER + lane / C);
-                const bool valid = r != NONE;
-                const size_t from = valid ? (size_t)r * S::ROW : 0;
-                const uint32_t to = at + (D == 256 && (it & 1) ? piece_at ^ 64 : piece_at) + it * PER * S::ROW;
-                copy_async<16>(to, k_from + from, valid);
-                copy_async<16>(to + S::CODES, v_from + from, valid);
+                for (int it = 0; it < C; it++) {
+                    const size_t from = (size_t)__shfl_sync(0xffffffffu, row, it * PER + lane / C) * S::ROW;
+                    const uint32_t to = at + (D == 256 && (it & 1) ? piece_at ^ 64 : piece_at) + it * PER * S::ROW;
+                    copy_async<16>(to, k_from + from);
+                    copy_async<16>(to + S::CODES, v_from + from);
+                }
+                copy_async<S::SROW>(at + scale_at, p.k_scales + (size_t)row * S::SROW);
+                copy_async<S::SROW>(at + scale_at + S::SCALES, p.v_scales + (size_t)row * S::SROW);
+            } else {   // the last tile, or a bad page: zeros for the rows that are not there
+#pragma unroll
+                for (int it = 0; it < C; it++) {
+                    const uint32_t r = __shfl_sync(0xffffffffu, row, it * PER + lane / C);
+                    const size_t from = r != NONE ? (size_t)r * S::ROW : 0;
+                    const uint32_t to = at + (D == 256 && (it & 1) ? piece_at ^ 64 : piece_at) + it * PER * S::ROW;
+                    copy_async<16>(to, k_from + from, r != NONE);
+                    copy_async<16>(to + S::CODES, v_from + from, r != NONE);
+                }
+                const size_t from = row != NONE ? (size_t)row * S::SROW : 0;
+                copy_async<S::SROW>(at + scale_at, p.k_scales + from, row != NONE);
+                copy_async<S::SROW>(at + scale_at + S::SCALES, p.v_scales + from, row != NONE);
             }
-            const bool valid = row != NONE;
-            const size_t from = valid ? (size_t)row * S::SROW : 0;
-            copy_async<S::SROW>(at + scale_at, p.k_scales + from, valid);
-            copy_async<S::SROW>(at + scale_at + S::SCALES, p.v_scales + from, valid);
         }
         asm volatile("cp.async.commit_group;");
     };
@@ -209,7 +232,8 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     for (int i = 0; i < S::STAGES - 1; i++) issue(i < tiles, ahead[i], i * S::STAGE);
     uint32_t row_ahead = ahead[S::STAGES - 1];
 
-    // q as B fragments in shared memory: [8 rows][step][lane][hi 0, hi 1, lo 0, lo 1]
+    // q as B fragments in shared memory: [8 rows][step][lane][hi 0, hi 1, lo 0, lo 1]; packed: [step][lane][2], columns 0-3
+    // hi, 4-7 lo
     for (int c = warp; c < COLS; c += WARPS) {
         constexpr int N = D / 32;
         const int ci = block * COLS + c;
@@ -233,8 +257,14 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
             const float y = x[i] * down;
             const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
             const int at = ((((c >> 3) * S::STEPS + step) * 32 + (c & 7) * 4 + owner) * 4 + (in & 1)) * 2 + ((in >> 2) & 1);
-            frag[at] = hi;
-            frag[at + 4] = lo;
+            if (PACK) {
+                const int at2 = ((step * 32 + c * 4 + owner) * 2 + (in & 1)) * 2 + ((in >> 2) & 1);
+                frag[at2] = hi;
+                frag[at2 + 64] = lo;   // 16 lanes on
+            } else {
+                frag[at] = hi;
+                frag[at + 4] = lo;
+            }
         }
     }
     __syncthreads();
@@ -247,8 +277,9 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 #pragma unroll
             for (int r = 0; r < 4; r++) o[nt][j][r] = 0.f;
 #pragma unroll
-    for (int r = 0; r < R; r++) { m[r] = -INFINITY; l[r] = 0.f; cs[r] = col_scale[2 * t + (r & 1) + (r >> 1) * 8]; }
+    for (int r = 0; r < R; r++) { m[r] = -INFINITY; l[r] = 0.f; cs[r] = col_scale[row_at(r)]; }
     const uint4* q_frag = reinterpret_cast<const uint4*>(smem) + lane;
+    const uint2* q_pack = reinterpret_cast<const uint2*>(smem) + lane;
 
     // this thread's pieces of a stage: K rows n * 8 + g (channels t D/4 ...), V rows 16 kb + 2t + {0, 1, 8, 9} (channels
     // g D/8 ...); rows 8 apart have the same permutation
@@ -293,18 +324,35 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int x = 0; x < 8; x++) a[nt][x >> 2][x & 3] = 0.f;
+        Scale pair[4][D == 256 ? 2 : 1];           // factors of two groups
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            const uint8_t* at = st + ks_at + n * 8 * S::SROW;
+            if constexpr (D == 64) pair[n][0] = scale_of(kv_scales_to_half(*at));
+            else if constexpr (D == 128) pair[n][0] = scale_of(kv_scales_to_half(*reinterpret_cast<const uint16_t*>(at)));
+            else {
+                const uint32_t v = *reinterpret_cast<const uint32_t*>(at);
+                pair[n][0] = scale_of(kv_scales_to_half(v & 0xffff));
+                pair[n][1] = scale_of(kv_scales_to_half(v >> 16));
+            }
+        }
 #pragma unroll
         for (int gr = 0; gr < D / 64; gr++) {      // groups of this thread's channels, two words each
             Scale sc[4];
 #pragma unroll
-            for (int n = 0; n < 4; n++) sc[n] = scale_of(kv_scales_to_half((uint32_t)st[ks_at + n * 8 * S::SROW + gr] * 0x101u));
+            for (int n = 0; n < 4; n++) sc[n] = half_of(pair[n][gr / 2], gr & 1);
 #pragma unroll
             for (int wi = 2 * gr; wi < 2 * gr + 2; wi++) {
                 uint4 f[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int u = 0; u < 2; u++) f[nt][u] = q_frag[(nt * S::STEPS + 2 * wi + u) * 32];
+                    for (int u = 0; u < 2; u++) {
+                        if constexpr (PACK) {
+                            const uint2 v = q_pack[(2 * wi + u) * 32];
+                            f[nt][u] = make_uint4(v.x, v.y, 0, 0);
+                        } else f[nt][u] = q_frag[(nt * S::STEPS + 2 * wi + u) * 32];
+                    }
 #pragma unroll
                 for (int kb = 0; kb < 2; kb++) {
                     uint32_t h[4], h8[4];
@@ -316,7 +364,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             mma(a[nt][kb], ka, f[nt][u].x, f[nt][u].y);
-                            mma(a[nt][kb], ka, f[nt][u].z, f[nt][u].w);
+                            if (!PACK) mma(a[nt][kb], ka, f[nt][u].z, f[nt][u].w);
                         }
                     }
                 }
@@ -355,12 +403,17 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
             poison = __reduce_or_sync(0xffffffffu, poison);
         }
 
+        if (PACK) {   // hi + lo columns
+#pragma unroll
+            for (int x = 0; x < 8; x++) a[0][x >> 2][x & 3] += __shfl_xor_sync(0xffffffffu, a[0][x >> 2][x & 3], 2);
+        }
+
         // ---- weights. Value x of a row: key key0 + 16 (x >> 1) + 8 (x & 1) + g
         float sv[R][4], top[R];
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int x = 0; x < 4; x++) sv[r][x] = a[r >> 1][x >> 1][2 * (x & 1) + (r & 1)] * cs[r];
+            for (int x = 0; x < 4; x++) sv[r][x] = a[r >> 1][x >> 1][2 * (x & 1) + (r & 1)];   // times cs[r]: log2 units
         if (key0 + TILE > least) {
 #pragma unroll
             for (int r = 0; r < R; r++)
@@ -371,7 +424,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
         bool raise = false;
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            top[r] = fmaxf(fmaxf(sv[r][0], sv[r][1]), fmaxf(sv[r][2], sv[r][3]));
+            top[r] = fmaxf(fmaxf(sv[r][0], sv[r][1]), fmaxf(sv[r][2], sv[r][3])) * cs[r];
             raise = raise || top[r] > m[r] + RAISE;
         }
         if (__any_sync(0xffffffffu, raise)) {   // some key exceeds its row's maximum by enough
@@ -402,7 +455,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
                 const float base = m[r] == -INFINITY ? 0.f : m[r] - P_BIAS;
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
-                    pw[u][x] = ex2(sv[r][x] - base);
+                    pw[u][x] = ex2(fmaf(sv[r][x], cs[r], -base));
                     if (poison && (poison >> (8 * x + g) & 1) && key0 + 8 * x + g < limit[r]) pw[u][x] = NAN;
                     l[r] += pw[u][x];
                 }
@@ -410,8 +463,9 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 #pragma unroll
             for (int x = 0; x < 4; x++) {
                 split(pw[0][x], pw[1][x], hi[nt][x], lo[nt][x]);
+                if (PACK) hi[nt][x] = t < 2 ? hi[nt][x] : lo[nt][x];
                 hi[nt][x] = transpose8(hi[nt][x]);
-                lo[nt][x] = transpose8(lo[nt][x]);
+                if (!PACK) lo[nt][x] = transpose8(lo[nt][x]);
             }
         }
 
@@ -448,7 +502,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             mma(o[nt][4 * wi + 2 * half + j], va, hi[nt][2 * kb], hi[nt][2 * kb + 1]);
-                            mma(o[nt][4 * wi + 2 * half + j], va, lo[nt][2 * kb], lo[nt][2 * kb + 1]);
+                            if (!PACK) mma(o[nt][4 * wi + 2 * half + j], va, lo[nt][2 * kb], lo[nt][2 * kb + 1]);
                         }
                     }
                 }
@@ -462,16 +516,21 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     for (int r = 0; r < R; r++) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
-        const int c = 2 * t + (r & 1) + (r >> 1) * 8;
+        const int c = row_at(r);
         if (g == 0) { sm_m[warp][c] = m[r]; sm_l[warp][c] = l[r]; }
+    }
+    if (PACK) {
+#pragma unroll
+        for (int x = 0; x < D / 4; x++) o[0][x >> 2][x & 3] += __shfl_xor_sync(0xffffffffu, o[0][x >> 2][x & 3], 2);
     }
     __syncthreads();   // every ring is idle
     float* so = reinterpret_cast<float*>(smem + S::Q_BYTES);
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        float* at = so + (warp * COLS + 2 * t + (r & 1) + (r >> 1) * 8) * S::O_LD + g * (D / 8);
+        float* at = so + (warp * COLS + row_at(r)) * S::O_LD + g * (D / 8);
 #pragma unroll
         for (int j = 0; j < D / 16; j += 2)
+            if (!PACK || t < 2)
             *reinterpret_cast<float4*>(at + 2 * j) = make_float4(o[r >> 1][j][r & 1], o[r >> 1][j][2 + (r & 1)],
                                                                  o[r >> 1][j + 1][r & 1], o[r >> 1][j + 1][2 + (r & 1)]);
     }
@@ -565,13 +624,21 @@ lancius_error bad(lancius_error e) { lancius_set_error(e); return e; }
 
 int row_blocks(int rows) { return rows > 8 ? (rows + 15) / 16 : 1; }
 
-// Chunks: about two rounds of the CTAs that fit on the GPU (a longer chunk wastes the end of the last round, a shorter
-// one spends more on its start and on joining), a multiple of one tile per warp.
+template <int D>
+int resident(int rows) { return rows <= 8 ? Shape<D, 8>::RESIDENT : Shape<D, 16>::RESIDENT; }
+
+// Keys per CTA. Few keys: every CTA that fits on the GPU gets one chunk (131072 keys of one sequence, 8 heads: 47.5 us in
+// one round of CTAs, 54.9 in two, 66.7 in three). Many keys: rounds of at most 1536, as short ones cost more starts
+// and joins and long ones an idle end (32 sequences of up to 8192 keys, 8 heads: 85.7 us with 256 keys, 70 with 1024 to
+// 1536, 74.9 with 2048). Sequences of a batch are taken as three quarters of the longest. A multiple of one tile per
+// warp.
 Split plan(const KvPagesDev& p, const KvBatchDev& b, int D, int group) {
-    const int per_sm = D == 256 ? Shape<256, false>::RESIDENT : D == 128 ? Shape<128, false>::RESIDENT : Shape<64, false>::RESIDENT;
-    const size_t ctas = (size_t)b.n_seqs * p.heads * row_blocks(group * b.max_new), len = b.max_len > 0 ? b.max_len : 1;
-    const size_t slots = 2 * (size_t)LCU_SMS * per_sm;
-    size_t chunk = (len * ctas + slots - 1) / slots;
+    const int rows = group * b.max_new;
+    const size_t slots = (size_t)LCU_SMS * (D == 256 ? resident<256>(rows) : D == 128 ? resident<128>(rows) : resident<64>(rows));
+    const size_t ctas = (size_t)b.n_seqs * p.heads * row_blocks(rows), len = b.max_len > 0 ? b.max_len : 1;
+    const size_t keys = len * ctas / 4 * (b.n_seqs > 1 ? 3 : 4);
+    size_t chunk = (keys + slots - 1) / slots;
+    if (chunk > MAX_CHUNK) chunk /= (chunk + 1535) / 1536;
     constexpr size_t STEP = TILE * WARPS;
     chunk = (chunk + STEP - 1) / STEP * STEP;
     if (chunk < STEP) chunk = STEP;
@@ -589,14 +656,14 @@ lancius_error check_call(const lcu_kv_pages* pages, const lcu_kv_batch* batch, s
     return LANCIUS_ERROR_OK;
 }
 
-template <int D, bool WIDE>
+template <int D, int ROWS>
 lancius_error launch(float* out, const float* q, size_t q_ld, int hq, const KvPagesDev& p, const KvBatchDev& b, Split sp,
                      float* part_o, float2* part_ml, cudaStream_t st) {
-    using S = Shape<D, WIDE>;
-    cudaError_t ce = cudaFuncSetAttribute(k_attn_paged<D, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    using S = Shape<D, ROWS>;
+    cudaError_t ce = cudaFuncSetAttribute(k_attn_paged<D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (ce != cudaSuccess) return lcu_check_cuda(ce);
     const dim3 grid((unsigned)(sp.splits * row_blocks(hq / p.heads * b.max_new)), (unsigned)p.heads, (unsigned)b.n_seqs);
-    k_attn_paged<D, WIDE><<<grid, THREADS, S::SMEM, st>>>(out, q, q_ld, hq, p, b, (float)(1.4426950408889634 / sqrt((double)D)), sp,
+    k_attn_paged<D, ROWS><<<grid, THREADS, S::SMEM, st>>>(out, q, q_ld, hq, p, b, (float)(1.4426950408889634 / sqrt((double)D)), sp,
                                                           part_o, part_ml);
     lcu_note_launch();
     if (sp.splits == 1) return lcu_launch_status();
@@ -618,6 +685,16 @@ lancius_error launch(float* out, const float* q, size_t q_ld, int hq, const KvPa
     }
     lcu_note_launch();
     return lcu_launch_status();
+}
+
+// rows of a key head: up to 4 fit one operand with both halves of q (half the MMAs), up to 8 one operand per half
+template <int D>
+lancius_error launch_rows(float* out, const float* q, size_t q_ld, int hq, const KvPagesDev& p, const KvBatchDev& b, Split sp,
+                          float* part_o, float2* part_ml, cudaStream_t st) {
+    const int rows = hq / p.heads * b.max_new;
+    if (rows <= 4) return launch<D, 4>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
+    if (rows <= 8) return launch<D, 8>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
+    return launch<D, 16>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
 }
 
 }  // namespace
@@ -659,14 +736,10 @@ lancius_error lcu_attention_paged(float* out, const float* q, size_t q_ld, size_
         part_o = static_cast<float*>(workspace);
         part_ml = reinterpret_cast<float2*>(part_o + rows * D);
     }
-    const bool wide = hq / p.heads * b.max_new > 8;   // more rows than one MMA's hi/lo halves hold
     cudaStream_t st = lcu_as_stream(stream);
-    if (D == 64) return wide ? launch<64, true>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st)
-                             : launch<64, false>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
-    if (D == 128) return wide ? launch<128, true>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st)
-                              : launch<128, false>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
-    return wide ? launch<256, true>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st)
-                : launch<256, false>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
+    if (D == 64) return launch_rows<64>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
+    if (D == 128) return launch_rows<128>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
+    return launch_rows<256>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
 }
 
 }  // extern "C"
