@@ -6,140 +6,254 @@
 // Angles, their sines and the rotation are in FP64 and rounded to FP32 once: an FP32 angle of
 // position 100000 is off by 0.004 rad, and a rounding border crossed by one ulp changes a stored
 // value by a whole step. One CTA computes the D/2 sines of its token once for all heads.
-// Both divisions are IEEE (__fdiv_rn): max|x| / 7 then rounds to the right side of every e4m3
-// border and x / scale to the right side of every half, since 7 * border and scale * half are FP32
-// numbers, and a number next to them differs by more than half a step of the quotient.
+// Roundings are those of exact quotients, although the fast path multiplies with reciprocals: where the product is so
+// near a border that it could lie on the wrong side (a relative 2^-22 for max|x| / 7, 2^-18 of a step for x / scale),
+// the group takes IEEE divisions, and those do not err: 7 * border and scale * half are FP32 numbers, and a number next
+// to one differs by more than half a step of the quotient.
 //
-// Bound: HBM, q + k + v read and q written in FP32, 0.56 bytes a cached element. Four adjacent
-// threads hold one 16-channel group as float4s, so loads are 512 contiguous bytes a warp, a
-// group's maximum takes two shuffles and its codes are written as 64-byte runs.
+// Bound: HBM, q + k + v read and q written in FP32, 0.56 bytes a cached element. One warp works on one token (or on a
+// part of its rows, when tokens are few): a lane keeps 8 channels and their four sines and walks down the rows of q, k
+// and v, so that two neighbours hold a 16-channel group and a warp reads 1024 contiguous bytes. Four channels a lane
+// took 142 instructions per 128 elements, and the kernel was bound by their issue.
 #include "kv_paged.cuh"
 #include <math.h>
 
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, WARPS = THREADS / 32;
 
 __device__ int g_kv_fault = 0;
 
-// sequence of token t, or -1 for a row that belongs to none (every thread of the block gets it)
-__device__ int find_sequence(const KvBatchDev& b, int t) {
-    if (!b.start) return t < b.n_seqs ? t : -1;
-    int before = 0;   // sequences that start at or before t; the last of them holds it (earlier ones are empty or end)
-    for (int i0 = 0; i0 < b.n_seqs; i0 += THREADS) {
-        const int i = i0 + threadIdx.x;
-        before += __syncthreads_count(i < b.n_seqs && b.start[i] <= t);
+// Where one warp works: token, sequence, position, and the cache row of (token, head 0) or -1.
+struct Place {
+    int token, part, pos;
+    long long row;      // of head 0
+    bool any;
+};
+
+__device__ __forceinline__ Place find_place(const KvPagesDev& p, const KvBatchDev& b, int part_shift) {
+    Place at;
+    const unsigned id = blockIdx.x * WARPS + threadIdx.x / 32;
+    const int lane = threadIdx.x & 31;
+    at.token = (int)(id >> part_shift);
+    at.part = (int)(id & ((1u << part_shift) - 1));
+    at.any = at.token < b.n_tokens;
+    int s = -1, end = 0;
+    if (!b.start) {
+        s = at.any && at.token < b.n_seqs ? at.token : -1;
+        end = s + 1;
+    } else {   // the last sequence that starts at or before the token holds it, unless it has ended
+        int before = 0;
+#pragma unroll 4
+        for (int i0 = 0; i0 < b.n_seqs; i0 += 32) {
+            const int i = i0 + lane;
+            before += __popc(__ballot_sync(0xffffffffu, i < b.n_seqs && b.start[i] <= at.token));
+        }
+        end = b.start[before];
+        if (before > 0 && at.any && at.token < end) s = before - 1;
     }
-    return before > 0 && t < b.start[before] ? before - 1 : -1;
+    at.any = s >= 0;
+    at.pos = at.any ? b.seq_len[s] - (end - at.token) : -1;
+    at.any = at.any && at.pos >= 0;
+    at.row = at.any ? kv_row(p, b, s, at.pos, 0) : -1;
+    return at;
+}
+// 8 floats by the widest access that their alignment allows (wide: 2: 32 bytes, 1: 16, 0: 4)
+__device__ __forceinline__ void load8(float (&x)[8], const float* p, int wide) {
+    if (wide == 2) {
+        asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
+                     : "l"(p));
+    } else if (wide == 1) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = p[i];
+    }
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8], int wide) {
+    if (wide == 2) {
+        asm volatile("st.global.v8.f32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]),
+                     "f"(x[5]), "f"(x[6]), "f"(x[7]), "l"(p) : "memory");
+    } else if (wide == 1) {
+        *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[i] = x[i];
+    }
+}
+__device__ __forceinline__ float max_abs(float a, float b) {   // up to its sign; NaN if either is
+    float r;
+    asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
-__device__ __forceinline__ float4 load4(const float* p, bool vec) {
-    return vec ? __ldcs(reinterpret_cast<const float4*>(p)) : make_float4(p[0], p[1], p[2], p[3]);
-}
-
-// x[4] of one thread, the group's other 12 in its neighbours: 4 codes (16 bits) and the scale byte
-__device__ __forceinline__ uint32_t quantise(float4 x, float unit, uint32_t& scale_byte) {
+// x[8] of one lane, the group's other 8 in its neighbour: 8 codes and the scale byte
+__device__ __forceinline__ uint32_t quantise(float (&x)[8], float unit, uint32_t& scale_byte) {
     if (unit != 1.f) {
-        x.x = __fdiv_rn(x.x, unit); x.y = __fdiv_rn(x.y, unit);
-        x.z = __fdiv_rn(x.z, unit); x.w = __fdiv_rn(x.w, unit);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = __fdiv_rn(x[i], unit);
     }
-    // the bits of |x| order like the numbers, with infinity and NaN above all of them
-    uint32_t m = max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu),
-                     max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
-    const uint32_t quad = 0xfu << (threadIdx.x & 28);
-    m = max(m, __shfl_xor_sync(quad, m, 1));
-    m = max(m, __shfl_xor_sync(quad, m, 2));
-    if (m >= 0x7f800000u) { scale_byte = 0x7f; return 0x8888; }
+    float m = max_abs(max_abs(max_abs(x[0], x[1]), max_abs(x[2], x[3])), max_abs(max_abs(x[4], x[5]), max_abs(x[6], x[7])));
+    m = fabsf(max_abs(m, __shfl_xor_sync(3u << (threadIdx.x & 30), m, 1)));
+    if (!(m < INFINITY)) { scale_byte = 0x7f; return 0x88888888u; }
+    // the scale of m (1 -+ 2^-22) / 7: where they differ, of the quotient itself
     uint16_t s2;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(s2) : "f"(0.f), "f"(__fdiv_rn(__uint_as_float(m), 7.f)));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(s2) : "f"(m * (0.14285714924335480f * (1 + 0x1p-22f))), "f"(m * (0.14285714924335480f * (1 - 0x1p-22f))));
+    if ((s2 & 0xff) != s2 >> 8) asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(s2) : "f"(0.f), "f"(__fdiv_rn(m, 7.f)));
     scale_byte = s2 & 0xff;
-    if (!scale_byte) return 0x8888;   // the whole group is below half of the smallest scale
+    if (!scale_byte) return 0x88888888u;   // the whole group is below half of the smallest scale
     const float s = kv_scale(scale_byte);
-    auto code = [s](float y) { return (uint32_t)(min(7, max(-7, __float2int_rn(__fdiv_rn(y, s)))) + 8); };
-    return code(x.x) | code(x.y) << 4 | code(x.z) << 8 | code(x.w) << 12;
+    float inv;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    constexpr float MAGIC = 12582912.f;   // 1.5 * 2^23: y + MAGIC - MAGIC is y rounded
+    float r[8], off = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float y = x[i] * inv;
+        r[i] = (y + MAGIC) - MAGIC;
+        off = fmaxf(off, fabsf(y - r[i]));
+    }
+    // scales of at least 2^-6 have all their bits, so |x / scale| < 7.5
+    if (!(off < 0.5f - 0x1p-18f && scale_byte >= 8 && scale_byte < 0x7e)) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) r[i] = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -7.f), 7.f);
+    }
+    // four codes are the digits of a number below 2^16; 2^23 + it has them in its low bits
+    auto four = [&](int i) {
+        return __float_as_uint(fmaf(fmaf(fmaf(r[i + 3], 16.f, r[i + 2]), 16.f, r[i + 1]), 16.f, r[i]) + (8388608.f + 0x8888));
+    };
+    return __byte_perm(four(0), four(4), 0x5410);
 }
 
-// grid.x = token, grid.y = parts of its (Hq + 2 Hkv) D / 4 float4s
+// 2^part_shift warps per token, each takes every so manieth set of rows
 template <int D>
-__global__ void __launch_bounds__(THREADS) k_kv_append(KvPagesDev p, KvBatchDev b, float* q_out, const float* q,
+__global__ void __launch_bounds__(THREADS, 4) k_kv_append(KvPagesDev p, KvBatchDev b, int part_shift, float* q_out, const float* q,
                                                        size_t q_ld, int hq, const float* __restrict__ k, size_t k_ld,
                                                        const float* __restrict__ v, size_t v_ld, double log2_base, int rotate,
-                                                       int q_vec, int k_vec, int v_vec) {
-    __shared__ double2 turn[D / 2];   // (cos, sin)
-    const int t = blockIdx.x;
-    const int s = find_sequence(b, t);
-    if (s < 0) return;
-    const int pos = b.seq_len[s] - ((b.start ? b.start[s + 1] : s + 1) - t);
-    if (pos < 0) return;
-    if (rotate && threadIdx.x < D / 2) {
-        double sn, cs;
-        sincos((double)pos * exp2(-(double)(2 * threadIdx.x) / D * log2_base), &sn, &cs);
-        turn[threadIdx.x] = make_double2(cs, sn);
+                                                       int wide) {
+    __shared__ double2 turn[WARPS][4][D / 8];         // (cos, sin) of pair 4e + i at [i][e]
+    constexpr int C = D / 8, ROWS = 32 / C, U = 2;    // lanes of a row, rows a warp takes at once, rows in flight
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, e = lane % C;
+    const unsigned id = blockIdx.x * WARPS + warp;
+    const size_t t = id >> part_shift;                // the token, if there is one
+    const int step = ROWS << part_shift, rows = hq + 2 * p.heads;   // of q, then k, then v
+    int row = (int)(id & ((1u << part_shift) - 1)) * ROWS + lane / C;
+    const float* qs = q + t * q_ld + 8 * e;
+    const float* ks = k + t * k_ld + 8 * e - (size_t)hq * D;
+    const float* vs = v + t * v_ld + 8 * e - (size_t)(hq + p.heads) * D;
+    auto fetch = [&](float (&x)[8], int r) {
+        if (r < rows) load8(x, (r < hq ? qs : r < hq + p.heads ? ks : vs) + (size_t)r * D, wide);
+    };
+    float x[U][8];
+    if (t < (size_t)b.n_tokens) {                     // while the token's place is looked up
+#pragma unroll
+        for (int u = 0; u < U; u++) fetch(x[u], row + u * step);
     }
-    __syncthreads();
-    constexpr int C = D / 4;   // float4s of a row
-    const int rows = hq + 2 * p.heads;
-    for (int c = blockIdx.y * THREADS + threadIdx.x; c < rows * C; c += gridDim.y * THREADS) {
-        const int row = c / C, e = c % C;
-        const bool is_q = row < hq, is_v = row >= hq + p.heads;
-        const int head = is_q ? row : is_v ? row - hq - p.heads : row - hq;
-        const float* src = is_q ? q + (size_t)t * q_ld : is_v ? v + (size_t)t * v_ld : k + (size_t)t * k_ld;
-        float4 x = load4(src + (size_t)head * D + 4 * e, is_q ? q_vec : is_v ? v_vec : k_vec);
-        if (rotate && !is_v) {
-            const double2 a = turn[2 * e], z = turn[2 * e + 1];
-            const double x0 = x.x, x1 = x.y, x2 = x.z, x3 = x.w;
-            x.x = (float)(x0 * a.x - x1 * a.y); x.y = (float)(x0 * a.y + x1 * a.x);
-            x.z = (float)(x2 * z.x - x3 * z.y); x.w = (float)(x2 * z.y + x3 * z.x);
+    const Place at = find_place(p, b, part_shift);
+    if (!at.any) return;
+    if (at.row < 0 && lane == 0) g_kv_fault = 1;
+    if (rotate) {
+#pragma unroll
+        for (int i = lane; i < D / 2; i += 32) {
+            double sn, cs;
+            sincos((double)at.pos * exp2(-(double)(2 * i) / D * log2_base), &sn, &cs);
+            turn[warp][i % 4][i / 4] = make_double2(cs, sn);
         }
-        if (is_q) {
-            float* dst = q_out + (size_t)t * hq * D + (size_t)head * D + 4 * e;
-            if (q_vec) *reinterpret_cast<float4*>(dst) = x;
-            else { dst[0] = x.x; dst[1] = x.y; dst[2] = x.z; dst[3] = x.w; }
-            continue;
+        __syncwarp();
+    }
+    float* qd = q_out + t * hq * D + 8 * e;
+    auto handle = [&](float (&y)[8], int r) {
+        const bool is_v = r >= hq + p.heads;
+        if (rotate && !is_v) {   // not when there is nothing to do: infinities stay
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const double2 a = turn[warp][i][e];
+                const double y0 = y[2 * i], y1 = y[2 * i + 1];
+                y[2 * i] = (float)(y0 * a.x - y1 * a.y);
+                y[2 * i + 1] = (float)(y0 * a.y + y1 * a.x);
+            }
         }
-        uint32_t sb;
-        const uint32_t codes = quantise(x, is_v ? p.v_unit : p.k_unit, sb);
-        const long long at = kv_row(p, b, s, pos, head);
-        if (at < 0) { g_kv_fault = 1; continue; }
-        *reinterpret_cast<uint16_t*>((is_v ? p.v_codes : p.k_codes) + at * (D / 2) + 2 * e) = (uint16_t)codes;
-        if ((e & 3) == 0) (is_v ? p.v_scales : p.k_scales)[at * (D / 16) + (e >> 2)] = (uint8_t)sb;
+        if (r < hq) {            // may be q's own place: a lane has read it, and only it does
+            store8(qd + (size_t)r * D, y, wide);
+        } else if (at.row >= 0) {
+            uint32_t sb;
+            const uint32_t c = quantise(y, is_v ? p.v_unit : p.k_unit, sb);
+            const size_t to = (size_t)at.row + ((size_t)(r - hq - (is_v ? p.heads : 0)) << p.page_shift);
+            *reinterpret_cast<uint32_t*>((is_v ? p.v_codes : p.k_codes) + to * (D / 2) + 4 * e) = c;
+            if ((e & 1) == 0) (is_v ? p.v_scales : p.k_scales)[to * (D / 16) + (e >> 1)] = (uint8_t)sb;
+        }
+    };
+    while (row < rows) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (row < rows) {
+                handle(x[u], row);
+                fetch(x[u], row + U * step);
+                row += step;
+            }
     }
 }
 
 template <int D>
 __global__ void __launch_bounds__(THREADS) k_kv_read(float* __restrict__ k_out, float* __restrict__ v_out, KvPagesDev p,
-                                                     KvBatchDev b) {
-    const int t = blockIdx.x;
-    const int s = find_sequence(b, t);
-    if (s < 0) return;
-    const int pos = b.seq_len[s] - ((b.start ? b.start[s + 1] : s + 1) - t);
-    if (pos < 0) return;
-    constexpr int C = D / 4;
-    for (int c = blockIdx.y * THREADS + threadIdx.x; c < 2 * p.heads * C; c += gridDim.y * THREADS) {
-        const int row = c / C, e = c % C;
-        const bool is_v = row >= p.heads;
-        const int head = is_v ? row - p.heads : row;
-        const long long at = kv_row(p, b, s, pos, head);
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (at < 0) {
-            g_kv_fault = 1;
-        } else {
-            const uint32_t c = *reinterpret_cast<const uint16_t*>((is_v ? p.v_codes : p.k_codes) + at * (D / 2) + 2 * e);
-            const float sc = kv_scale((is_v ? p.v_scales : p.k_scales)[at * (D / 16) + (e >> 2)]);
-            auto value = [&](int i) { return (float)((int)(c >> (4 * i) & 15) - 8) * sc * (is_v ? p.v_unit : p.k_unit); };
-            x = make_float4(value(0), value(1), value(2), value(3));
+                                                     KvBatchDev b, int part_shift, int wide) {
+    constexpr int C = D / 8, ROWS = 32 / C, U = 4;
+    const int lane = threadIdx.x % 32, e = lane % C;
+    const Place at = find_place(p, b, part_shift);
+    if (!at.any) return;
+    if (at.row < 0 && lane == 0) g_kv_fault = 1;
+    const int step = ROWS << part_shift;
+    int row = at.part * ROWS + lane / C;   // of k, then v
+    auto get = [&](float* out, const uint8_t* codes, const uint8_t* scales, float unit) {
+        out += (size_t)at.token * p.heads * D + 8 * e;
+        if (at.row >= 0) {
+            codes += at.row * (D / 2) + 4 * e;
+            scales += at.row * (D / 16) + (e >> 1);
         }
-        *reinterpret_cast<float4*>((is_v ? v_out : k_out) + ((size_t)t * p.heads + head) * D + 4 * e) = x;
-    }
+        while (row < p.heads) {
+            uint32_t c[U], sb[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const size_t r = (size_t)(row + u * step) << p.page_shift;
+                const bool there = row + u * step < p.heads && at.row >= 0;
+                c[u] = there ? __ldcs(reinterpret_cast<const uint32_t*>(codes + r * (D / 2))) : 0;
+                sb[u] = there ? scales[r * (D / 16)] : 0;   // scale 0 reads as zeros
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (row < p.heads) {
+                    const float sc = kv_scale(sb[u]);
+                    float x[8];
+                    // n or'ed into the mantissa of 2^23 is 2^23 + n; (n - 8) * scale is exact, the unit rounds
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[i] = (__uint_as_float(0x4b000000u | (c[u] >> (4 * i) & 15)) - 8388616.f) * sc * unit;
+                    store8(out + (size_t)row * D, x, wide);
+                    row += step;
+                }
+        }
+        row -= p.heads;
+    };
+    get(k_out, p.k_codes, p.k_scales, p.k_unit);
+    get(v_out, p.v_codes, p.v_scales, p.v_unit);
 }
 
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 lancius_error bad(lancius_error e) { lancius_set_error(e); return e; }
 
-// CTAs per token: enough for about two CTAs per SM when tokens are few, at most one pass each
-unsigned parts(int tokens, int float4s) {
-    const int most = (float4s + THREADS - 1) / THREADS, want = (2 * LCU_SMS + tokens - 1) / tokens;
-    return (unsigned)(want < most ? want : most);
+// Warps per token, as a power of two: few tokens are spread over about 8 warps per SM (each repeats the sines), as far as
+// there are rows
+int part_shift(int tokens, int rows, int rows_at_once) {
+    int shift = 0;
+    while (((size_t)tokens << shift) < 8 * LCU_SMS && (rows_at_once << shift) < rows) shift++;
+    return shift;
+}
+unsigned part_blocks(int tokens, int shift) { return (unsigned)((((size_t)tokens << shift) + WARPS - 1) / WARPS); }
+// widest access to rows `ld` floats apart (load8, store8)
+int width(const void* p, size_t ld) {
+    return (uintptr_t)p % 32 == 0 && ld % 8 == 0 ? 2 : (uintptr_t)p % 16 == 0 && ld % 4 == 0 ? 1 : 0;
 }
 
 }  // namespace
@@ -197,14 +311,14 @@ lancius_error lcu_kv_append_paged(const lcu_kv_pages* pages, const lcu_kv_batch*
     if (n_q_heads && q == q_out && q_ld != n_q_heads * D) return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
     const int rotate = rope_base > 0;
     const double lb = rotate ? log2(rope_base) : 0.0;
-    const int qv = aligned16(q) && aligned16(q_out) && q_ld % 4 == 0, kvec = aligned16(k) && k_ld % 4 == 0,
-              vvec = aligned16(v) && v_ld % 4 == 0;
+    int wide = n_q_heads ? min(width(q, q_ld), width(q_out, 0)) : 2;
+    wide = min(wide, min(width(k, k_ld), width(v, v_ld)));
     const int hq = (int)n_q_heads;
-    const dim3 grid((unsigned)b.n_tokens, parts(b.n_tokens, (hq + 2 * p.heads) * (int)D / 4));
+    const int shift = part_shift(b.n_tokens, hq + 2 * p.heads, 256 / (int)D);
+    const unsigned grid = part_blocks(b.n_tokens, shift);
     cudaStream_t st = lcu_as_stream(stream);
-    if (D == 64) k_kv_append<64><<<grid, THREADS, 0, st>>>(p, b, q_out, q, q_ld, hq, k, k_ld, v, v_ld, lb, rotate, qv, kvec, vvec);
-    else if (D == 128) k_kv_append<128><<<grid, THREADS, 0, st>>>(p, b, q_out, q, q_ld, hq, k, k_ld, v, v_ld, lb, rotate, qv, kvec, vvec);
-    else k_kv_append<256><<<grid, THREADS, 0, st>>>(p, b, q_out, q, q_ld, hq, k, k_ld, v, v_ld, lb, rotate, qv, kvec, vvec);
+    auto kernel = D == 64 ? k_kv_append<64> : D == 128 ? k_kv_append<128> : k_kv_append<256>;
+    kernel<<<grid, THREADS, 0, st>>>(p, b, shift, q_out, q, q_ld, hq, k, k_ld, v, v_ld, lb, rotate, wide);
     lcu_note_launch();
     return lcu_launch_status();
 }
@@ -217,13 +331,11 @@ lancius_error lcu_kv_read_paged(float* k_out, float* v_out, const lcu_kv_pages* 
     if (e != LANCIUS_ERROR_OK) return e;
     if (!b.n_seqs || !b.n_tokens) return LANCIUS_ERROR_OK;
     if (!k_out || !v_out) return bad(LANCIUS_ERROR_NULL_PTR);
-    if (!aligned16(k_out) || !aligned16(v_out)) return bad(LANCIUS_ERROR_UNSUPPORTED_DTYPE);
     const size_t D = pages->head_dim;
-    const dim3 grid((unsigned)b.n_tokens, parts(b.n_tokens, 2 * p.heads * (int)D / 4));
-    cudaStream_t st = lcu_as_stream(stream);
-    if (D == 64) k_kv_read<64><<<grid, THREADS, 0, st>>>(k_out, v_out, p, b);
-    else if (D == 128) k_kv_read<128><<<grid, THREADS, 0, st>>>(k_out, v_out, p, b);
-    else k_kv_read<256><<<grid, THREADS, 0, st>>>(k_out, v_out, p, b);
+    const int shift = part_shift(b.n_tokens, 2 * p.heads, 256 / (int)D);
+    const int wide = min(width(k_out, 0), width(v_out, 0));
+    auto kernel = D == 64 ? k_kv_read<64> : D == 128 ? k_kv_read<128> : k_kv_read<256>;
+    kernel<<<part_blocks(b.n_tokens, shift), THREADS, 0, lcu_as_stream(stream)>>>(k_out, v_out, p, b, shift, wide);
     lcu_note_launch();
     return lcu_launch_status();
 }
