@@ -22,6 +22,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 2048, LIST = THREADS, MAX_CLUSTER = 8;
+constexpr int SMALL = 256;   // candidates that one CTA finishes alone
 constexpr int BLOCK = 128;   // logits whose weights are summed as one in the draw, 4 a lane
 constexpr double FIXED = 17592186044416.0;   // 2^44
 constexpr size_t MAX_VOCAB = 262144;
@@ -35,32 +36,49 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
 struct Shared {
-    u64 mass[BINS];
-    uint32_t count[BINS];
+    uint32_t low[BINS], high[BINS];    // of a bin: its sum (counts in low alone)
     float warp_max[WARPS], warp_min[WARPS];
     u64 list[LIST], list_mass[LIST];   // key << 32 | ~index, so that larger means an earlier rank
     double power[16];
     u64 warp_sum[WARPS];
     double block_mass[MAX_BLOCKS], mass_here;
-    float max, min;
+    float max, min, tau;
     int at, found, bin, last;
-    uint32_t listed, members, tau;
-    u64 before, in_bin, total, ties;
+    uint32_t listed;
+    u64 slice_sum, before, in_bin, total;
 };
 
 struct Row {
     const float* x;     // this CTA's part, in shared memory, cleaned
-    int n, first;       // its length and the index of its first token
+    int padded, first;  // its length and the index of its first token
     float max, min;     // of the row, min over the finite ones
     double top, rate;   // max, log2(e) / t
     float nothing;      // weights are 0 below this logit
     const double* power;   // 2^(j/16), in shared memory
-    uint32_t tau;       // kept: key > tau, or key == tau and index <= last
+    bool fresh;         // the histogram is cleared
+    float tau;          // kept: logit > tau, or logit == tau and index <= last
     int last;
 };
 
-__device__ __forceinline__ bool kept(const Row& r, uint32_t key, int i) { return key > r.tau || (key == r.tau && r.first + i <= r.last); }
+constexpr int ALL = 0x7fffffff;
+__device__ __forceinline__ bool kept(const Row& r, float x, int i) { return x >= r.tau && (r.last == ALL || x > r.tau || r.first + i <= r.last); }
+// Calls use(logit, index in the part) for the kept logits of this CTA's part, 4 neighbours at a time per thread. The
+// part is padded with -infinity, which is never kept, to a multiple of BLOCK.
+template <typename Use>
+__device__ __forceinline__ void for_kept(const Row& r, Use use) {
+    const float4* x4 = reinterpret_cast<const float4*>(r.x);
+#pragma unroll 2
+    for (int j = threadIdx.x; j < r.padded / 4; j += THREADS) {
+        const float4 v = x4[j];
+        if (kept(r, v.x, 4 * j)) use(v.x, 4 * j);
+        if (kept(r, v.y, 4 * j + 1)) use(v.y, 4 * j + 1);
+        if (kept(r, v.z, 4 * j + 2)) use(v.z, 4 * j + 2);
+        if (kept(r, v.w, 4 * j + 3)) use(v.w, 4 * j + 3);
+    }
+}
 // exp((x - max) / t) as 2^z, z = n / 16 + f, |f| <= 1/32: a table of 2^(j/16) times the Taylor series of 2^f to f^6
 // (table-driven exponential, Tang 1989); the series' remainder is 5e-16. 13 FP64 instructions, where the library's
 // exp and a division took 124 of all kinds. Below 2^-1000 the
@@ -96,117 +114,195 @@ __device__ u64 block_scan(Shared& sh, u64 v) {
     __syncthreads();
     if (lane == 31) sh.warp_sum[warp] = v;
     __syncthreads();
-    u64 add = 0;
-    for (int w = 0; w < warp; w++) add += sh.warp_sum[w];
-    return v + add;
+    u64 add = lane < warp ? sh.warp_sum[lane] : 0;
+#pragma unroll
+    for (int o = WARPS / 2; o > 0; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
+    return v + __shfl_sync(0xffffffffu, add, 0);
 }
 
-// One histogram over the kept logits, bin_of(x, key) < BINS rising with the rank (or -1: not counted), and the bin in
-// which the running sum reaches the target: sh.bin, sh.before (sum before the bin, starting at `before`),
-// sh.in_bin, sh.members, sh.found. The target is made by target_of(total) from the sum of all bins.
+__device__ __forceinline__ void clear(Shared& sh) {
+    for (int i = threadIdx.x; i < BINS; i += THREADS) sh.low[i] = sh.high[i] = 0;
+    if (threadIdx.x == 0) sh.listed = 0;
+}
+
+// One histogram over the kept logits, of counts or masses, bin_of(x) < BINS rising with the rank (or -1: not counted), and
+// the bin in which the running sum, from `before` on, reaches the target, which target_of(total) makes from the sum of
+// all bins.
+struct Found {
+    bool any;
+    int bin;
+    u64 before, in_bin, total;   // sum before the bin, in it, of all bins
+};
 template <bool MASS, typename Bin, typename Target>
-__device__ void find_bin(cg::cluster_group& cl, Shared& sh, const Row& r, u64 before, Bin bin_of, Target target_of) {
-    const int tid = threadIdx.x, ranks = cl.num_blocks(), slice = BINS / ranks;
-    cl.sync();   // nobody reads the last histogram any more
-    for (int i = tid; i < BINS; i += THREADS) { sh.mass[i] = 0; sh.count[i] = 0; }
-    if (tid == 0) { sh.found = 0; sh.listed = 0; }
-    __syncthreads();
-    for (int i = tid; i < r.n; i += THREADS) {
-        const float x = r.x[i];
-        const uint32_t key = key_of(x);
-        if (!kept(r, key, i)) continue;
-        const int bin = bin_of(x, key);
-        if (bin < 0) continue;
-        atomicAdd(&sh.count[bin], 1u);
-        if (MASS) atomicAdd(&sh.mass[bin], fixed_weight(r, x));
+__device__ Found find_bin(cg::cluster_group& cl, Shared& sh, Row& r, u64 before, Bin bin_of, Target target_of) {
+    const int tid = threadIdx.x, lane = tid & 31, ranks = cl.num_blocks(), rank = cl.block_rank(), slice = BINS / ranks;
+    if (!r.fresh) {
+        cl.sync();   // nobody reads the last histogram any more
+        clear(sh);
+        __syncthreads();
     }
-    cl.sync();
-    if (ranks > 1) {   // each CTA adds up its slice of the bins, in place: nobody else reads that slice of its own
-        const int b0 = cl.block_rank() * slice;
-        for (int i = b0 + tid; i < b0 + slice; i += THREADS) {
-            uint32_t c = 0;
-            u64 m = 0;
-#pragma unroll
-            for (int k = 0; k < MAX_CLUSTER; k++)   // unrolled: the remote reads are in flight together
-                if (k < ranks) {
-                    const Shared* o = cl.map_shared_rank(&sh, k);
-                    c += o->count[i];
-                    if (MASS) m += o->mass[i];
-                }
-            sh.count[i] = c;
-            sh.mass[i] = m;
+    r.fresh = false;
+    for_kept(r, [&](float x, int) {
+        const int bin = bin_of(x);
+        if (bin < 0) return;
+        if (MASS) {   // two 32-bit atomics with a carry: shared memory has no 64-bit add
+            const u64 w = fixed_weight(r, x);
+            const uint32_t lo = (uint32_t)w, old = atomicAdd(&sh.low[bin], lo);
+            const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old);
+            if (hi) atomicAdd(&sh.high[bin], hi);
+        } else {
+            atomicAdd(&sh.low[bin], 1u);
         }
-        cl.sync();
-    }
-    // every CTA scans all bins
+    });
+    cl.sync();
+    // each CTA adds up its slice of the bins over the cluster and scans it, q neighbours a thread
+    const int b0 = rank * slice, q = max(1, slice / THREADS);
     constexpr int PER = BINS / THREADS;
     u64 v[PER], sum = 0;
-    uint32_t c[PER];
-    const Shared* owner = cl.map_shared_rank(&sh, PER * tid / slice);
 #pragma unroll
     for (int k = 0; k < PER; k++) {
-        c[k] = owner->count[PER * tid + k];
-        v[k] = MASS ? owner->mass[PER * tid + k] : c[k];
+        const int i = q * tid + k;
+        v[k] = 0;
+        if (k < q && i < slice) {
+            u64 x[MAX_CLUSTER];   // the remote reads are in flight together
+#pragma unroll
+            for (int c = 0; c < MAX_CLUSTER; c++) {
+                const Shared* o = cl.map_shared_rank(&sh, min(c, ranks - 1));
+                x[c] = c < ranks ? o->low[b0 + i] + (MASS ? (u64)o->high[b0 + i] << 32 : 0) : 0;
+            }
+#pragma unroll
+            for (int c = 0; c < MAX_CLUSTER; c++) v[k] += x[c];
+        }
         sum += v[k];
     }
     const u64 upto = block_scan(sh, sum);
-    if (tid == THREADS - 1) sh.total = upto;
-    __syncthreads();
-    const double target = target_of(sh.total);
-    u64 at = before + upto - sum;
+    if (tid == THREADS - 1) { sh.slice_sum = upto; sh.found = 0; }
+    cl.sync();
+    u64 slices = lane < ranks ? cl.map_shared_rank(&sh, lane % ranks)->slice_sum : 0;
+    u64 ahead = lane < rank ? slices : 0;
+#pragma unroll
+    for (int o = MAX_CLUSTER / 2; o > 0; o >>= 1) {
+        slices += __shfl_xor_sync(0xffffffffu, slices, o);
+        ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+    }
+    const u64 total = __shfl_sync(0xffffffffu, slices, 0);
+    const double target = target_of(total);
+    u64 at = before + __shfl_sync(0xffffffffu, ahead, 0) + upto - sum;
 #pragma unroll
     for (int k = 0; k < PER; k++) {
-        if ((double)at < target && (double)(at + v[k]) >= target) {   // one bin of one thread
-            sh.bin = PER * tid + k; sh.before = at; sh.in_bin = v[k]; sh.members = c[k]; sh.found = 1;
+        if ((double)at < target && (double)(at + v[k]) >= target) {   // one bin of one thread of one CTA
+            sh.bin = b0 + q * tid + k; sh.before = at; sh.in_bin = v[k]; sh.found = 1;
         }
         at += v[k];
     }
-    __syncthreads();
+    cl.sync();
+    const Shared* o = cl.map_shared_rank(&sh, lane % ranks);
+    const unsigned owners = __ballot_sync(0xffffffffu, o->found);
+    o = cl.map_shared_rank(&sh, owners ? __ffs(owners) - 1 : 0);
+    return Found{owners != 0, o->bin, o->before, o->in_bin, total};
 }
 
-// The kept logits with in(x, key) are at most LIST: ranks them and moves the cut to the one at which the sum reaches the
-// target.
-template <bool MASS, typename In>
-__device__ void finish_list(cg::cluster_group& cl, Shared& sh, Row& r, double target, In in) {
+// Puts a logit on the first CTA's list (its counter is cleared with the histogram).
+__device__ __forceinline__ void put(const Row& r, Shared* lead, int i, float x, u64 mass) {
+    const uint32_t to = atomicAdd(&lead->listed, 1u);
+    if (to >= LIST) return;
+    lead->list[to] = (u64)key_of(x) << 32 | (uint32_t)~(uint32_t)(r.first + i);
+    lead->list_mass[to] = mass;
+}
+
+// All of a list is on it (cluster barrier passed): the first CTA ranks it, starting from the sum `before`, and the cut moves
+// to the logit at which the sum reaches the target.
+template <bool MASS>
+__device__ void rank_list(cg::cluster_group& cl, Shared& sh, Row& r, u64 before, double target) {
     const int tid = threadIdx.x;
-    const u64 before = sh.before;
-    Shared* lead = cl.map_shared_rank(&sh, 0);   // its counter was zeroed before the histogram
-    for (int i = tid; i < r.n; i += THREADS) {
-        const float x = r.x[i];
-        const uint32_t key = key_of(x);
-        if (!kept(r, key, i) || !in(x, key)) continue;
-        const uint32_t to = atomicAdd(&lead->listed, 1u);
-        if (to >= LIST) continue;
-        lead->list[to] = (u64)key << 32 | (uint32_t)~(uint32_t)(r.first + i);
-        if (MASS) lead->list_mass[to] = fixed_weight(r, x);
-    }
-    cl.sync();
     if (cl.block_rank() == 0) {
-        const int n = min(sh.listed, (uint32_t)LIST);
+        const int n = sh.listed;
         if (tid < n) {
             const u64 me = sh.list[tid];
             u64 ahead = before;
+#pragma unroll 4
             for (int j = 0; j < n; j++)
                 if (sh.list[j] > me) ahead += MASS ? sh.list_mass[j] : 1;
             const u64 w = MASS ? sh.list_mass[tid] : 1;
-            if ((double)ahead < target && (double)(ahead + w) >= target) { sh.tau = (uint32_t)(me >> 32); sh.last = (int)~(uint32_t)me; }
+            if ((double)ahead < target && (double)(ahead + w) >= target) {
+                sh.tau = of_key((uint32_t)(me >> 32));
+                sh.last = (int)~(uint32_t)me;
+            }
         }
     }
     cl.sync();
+    const Shared* lead = cl.map_shared_rank(&sh, 0);
     r.tau = lead->tau;
     r.last = lead->last;
 }
 
-// Of the kept logits equal to `key`, the one that is the keep-th by index becomes the last.
-__device__ void finish_ties(cg::cluster_group& cl, Shared& sh, Row& r, uint32_t key, u64 keep) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int seg = ((r.n + WARPS - 1) / WARPS + 31) / 32 * 32, s0 = warp * seg, s1 = min(r.n, s0 + seg);
-    auto hits = [&](int i) {
-        const uint32_t k = i < s1 ? key_of(r.x[i]) : 0;
-        return __ballot_sync(0xffffffffu, i < s1 && k == key && kept(r, k, i));
+// Cuts within the kept logits with in(x), the sum before which is `before`. False: they are more than LIST; their number
+// is in the first CTA's `listed`.
+template <bool MASS, typename In>
+__device__ bool finish_list(cg::cluster_group& cl, Shared& sh, Row& r, u64 before, double target, In in) {
+    Shared* lead = cl.map_shared_rank(&sh, 0);
+    for_kept(r, [&](float x, int i) {
+        if (in(x)) put(r, lead, i, x, MASS ? fixed_weight(r, x) : 0);
+    });
+    cl.sync();
+    if (lead->listed > LIST) return false;
+    rank_list<MASS>(cl, sh, r, before, target);
+    return true;
+}
+
+// The kept logits with in(x) are at most SMALL and hold all of the top k: the first CTA ranks them, cuts by k and p
+// and draws. Masses are fixed point, as the list's order is anybody's.
+template <typename In>
+__device__ void finish_small(cg::cluster_group& cl, Shared& sh, const Row& r, int k, double p, double u, int32_t* token, In in) {
+    const int tid = threadIdx.x;
+    Shared* lead = cl.map_shared_rank(&sh, 0);
+    for_kept(r, [&](float x, int i) {
+        if (in(x)) put(r, lead, i, x, fixed_weight(r, x));
+    });
+    cl.sync();
+    if (cl.block_rank() != 0) return;   // only the first CTA's shared memory is used from here on
+    const int n = min(sh.listed, (uint32_t)LIST);
+    const bool mine = tid < n;
+    const u64 me = mine ? sh.list[tid] : 0, w = mine ? sh.list_mass[tid] : 0;
+    const int index = (int)~(uint32_t)me;
+    u64 ahead = 0;
+    int rank = 0;
+    if (mine)
+        for (int j = 0; j < n; j++)
+            if (sh.list[j] > me) { rank++; ahead += sh.list_mass[j]; }
+    bool keep = mine && rank < k;
+    auto sum = [&](u64 v) {
+        v = block_scan(sh, v);
+        if (tid == THREADS - 1) sh.total = v;
+        __syncthreads();
+        return sh.total;
     };
+    if (p < 1.0) {
+        const double target = fmax(p * (double)sum(keep ? w : 0), 0.5);
+        keep = keep && (double)ahead < target;
+    }
+    const double target = u * (double)sum(keep ? w : 0);
+    if (tid == 0) { sh.at = 0x7fffffff; sh.last = -1; }
+    if (mine && !keep) sh.list_mass[tid] = 0;
+    __syncthreads();
+    if (keep) {
+        u64 upto = 0;
+        for (int j = 0; j < n; j++)
+            if ((uint32_t)sh.list[j] >= (uint32_t)me) upto += sh.list_mass[j];   // indices up to this one
+        if (w && (double)upto > target) atomicMin(&sh.at, index);
+        if (w || rank == 0) atomicMax(&sh.last, index);
+    }
+    __syncthreads();
+    if (tid == 0) *token = sh.at < 0x7fffffff ? sh.at : sh.last;
+}
+
+// Of the kept logits equal to `value`, the one that is the keep-th by index becomes the last.
+__device__ void finish_ties(cg::cluster_group& cl, Shared& sh, Row& r, float value, u64 keep) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int seg = (r.padded / 32 + WARPS - 1) / WARPS * 32, s0 = warp * seg, s1 = min(r.padded, s0 + seg);
+    auto hits = [&](int i) { return __ballot_sync(0xffffffffu, r.x[i] == value && kept(r, r.x[i], i)); };
     u64 n = 0;
-    for (int i = s0 + lane; i - lane < s1; i += 32) n += __popc(hits(i));
+    for (int i = s0 + lane; i < s1; i += 32) n += __popc(hits(i));
     __syncthreads();
     if (lane == 0) sh.warp_sum[warp] = n;
     cl.sync();
@@ -217,7 +313,7 @@ __device__ void finish_ties(cg::cluster_group& cl, Shared& sh, Row& r, uint32_t 
     for (int o = 16; o > 0; o >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
     Shared* lead = cl.map_shared_rank(&sh, 0);
     if (ahead < keep && ahead + n >= keep) {
-        for (int i = s0 + lane; i - lane < s1; i += 32) {
+        for (int i = s0 + lane; i < s1; i += 32) {
             unsigned h = hits(i);
             const int c = __popc(h);
             if (ahead + c >= keep) {
@@ -229,51 +325,64 @@ __device__ void finish_ties(cg::cluster_group& cl, Shared& sh, Row& r, uint32_t 
         }
     }
     cl.sync();
-    r.tau = key;
+    r.tau = value;
     r.last = lead->last;
 }
 
-// Moves the row's cut to the rank at which the running count (MASS = false: k) or mass (p times the mass of what is
-// kept so far) is reached.
-template <bool MASS>
-__device__ void cut(cg::cluster_group& cl, Shared& sh, Row& r, int k, double p) {
-    double target = k;
-    auto first_target = [&](u64 total) { return MASS ? fmax(p * (double)total, 0.5) : (double)k; };
-    // bins of equal width in the logit, down to weights of e^-100
-    const float range = fminf(r.max - r.min, 144.f / (float)r.rate);
-    if (range > 0.f && range < INFINITY) {
-        const float per = (BINS - 1) / range;
-        auto bin_of = [&](float x, uint32_t) { return min(BINS - 1, __float2int_rz((r.max - x) * per)); };
-        find_bin<MASS>(cl, sh, r, 0, bin_of, first_target);
-        if (!sh.found) return;   // fewer than k, or all of the mass is wanted
-        if (sh.members <= LIST) {
-            target = first_target(sh.total);
-            const int bin = sh.bin;
-            finish_list<MASS>(cl, sh, r, target, [&](float x, uint32_t key) { return bin_of(x, key) == bin; });
-            return;
-        }
+// Bins of equal width in the logit, down to weights of 2^-144; false where the logits' range allows none.
+struct ValueBins {
+    float max, per;
+    __device__ bool make(const Row& r) {
+        const float range = fminf(r.max - r.min, 144.f / (float)r.rate);
+        max = r.max;
+        per = (BINS - 1) / range;
+        return range > 0.f && range < INFINITY && per < 1e30f;
     }
-    uint32_t lo = r.tau, hi = key_of(r.max);
+    __device__ __forceinline__ int operator()(float x) const { return min(BINS - 1, __float2int_rz((max - x) * per)); }
+};
+
+// Moves the row's cut to the rank at which the running count (MASS = false: k) or mass (p times the mass of what is
+// kept so far) is reached. With a count of few candidates it draws the token at once and returns true.
+template <bool MASS>
+__device__ bool cut(cg::cluster_group& cl, Shared& sh, Row& r, int k, double p, double u, int32_t* token) {
+    auto first_target = [&](u64 total) { return MASS ? fmax(p * (double)total, 0.5) : (double)k; };
+    ValueBins bin_of;
+    if (bin_of.make(r)) {
+        const Found f = find_bin<MASS>(cl, sh, r, 0, bin_of, first_target);
+        const int bin = f.any ? f.bin : BINS;
+        if (!MASS && (f.any ? f.before + f.in_bin : f.total) <= SMALL) {
+            finish_small(cl, sh, r, k, p, u, token, [&](float x) { return bin_of(x) <= bin; });
+            return true;
+        }
+        if (!f.any) return false;   // fewer than k, or all of the mass is wanted
+        if ((MASS || f.in_bin <= LIST) &&
+            finish_list<MASS>(cl, sh, r, f.before, first_target(f.total), [&](float x) { return bin_of(x) == bin; }))
+            return false;
+    }
+    uint32_t lo = key_of(r.tau), hi = key_of(r.max);
     u64 before = 0;
+    double target = 0.0;
     for (bool first = true;; first = false) {   // at most 3 rounds: 32 bits, 21, 10
         const int bits = max(0, 32 - __clz(hi - lo) - 11);
-        auto bin_of = [&](float, uint32_t key) { return key < lo || key > hi ? -1 : (int)((hi - key) >> bits); };
-        find_bin<MASS>(cl, sh, r, before, bin_of, [&](u64 total) { return first ? first_target(total) : target; });
-        if (!sh.found) return;
-        if (first) target = first_target(sh.total);
-        before = sh.before;
-        hi -= (uint32_t)sh.bin << bits;
+        auto key_bin = [&](float x) {
+            const uint32_t key = key_of(x);
+            return key < lo || key > hi ? -1 : (int)((hi - key) >> bits);
+        };
+        const Found f = find_bin<MASS>(cl, sh, r, before, key_bin, [&](u64 total) { return first ? first_target(total) : target; });
+        if (!f.any) return false;
+        if (first) target = first_target(f.total);
+        before = f.before;
+        hi -= (uint32_t)f.bin << bits;
         const uint32_t low = hi - ((1u << bits) - 1);
         if (low > lo && low <= hi) lo = low;
-        if (sh.members <= LIST) {
-            finish_list<MASS>(cl, sh, r, target, [&](float, uint32_t key) { return key >= lo && key <= hi; });
-            return;
-        }
+        if ((MASS || f.in_bin <= LIST || !bits) &&
+            finish_list<MASS>(cl, sh, r, before, target, [&](float x) { return key_of(x) >= lo && key_of(x) <= hi; }))
+            return false;
         if (bits) continue;
-        const double ties = (double)sh.members, each = (double)sh.in_bin / ties;
+        const double ties = (double)cl.map_shared_rank(&sh, 0)->listed, each = (double)f.in_bin / ties;
         const double need = MASS ? fmin(fmax(ceil((target - (double)before) / each), 1.0), ties) : target - (double)before;
-        finish_ties(cl, sh, r, hi, (u64)need);
-        return;
+        finish_ties(cl, sh, r, of_key(hi), (u64)need);
+        return false;
     }
 }
 
@@ -288,11 +397,13 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
     Row r;
     r.x = part_of_row;
     r.first = rank * part;
-    r.n = max(0, min(part, vocab - r.first));
+    const int n = max(0, min(part, vocab - r.first));
+    r.padded = (n + BLOCK - 1) / BLOCK * BLOCK;
     const float* src = logits + (size_t)row * ld + r.first;
     const float t = temperature ? temperature[row] : 1.f, mp = min_p ? min_p[row] : 0.f, p = top_p ? top_p[row] : 1.f;
     const int k = top_k ? top_k[row] : 0;
     const bool greedy = !(t > 0.f), cuts = !greedy && ((k > 0 && k < vocab) || p < 1.f);
+    const double rate = 1.4426950408889634074 / (double)t;
     float m = -INFINITY, lowest = INFINITY;   // lowest of the finite ones, where a cut will want it
     auto take = [&](float x) {
         x = clean(x);
@@ -300,14 +411,15 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
         if (cuts && x > -INFINITY) lowest = fminf(lowest, x);
         return x;
     };
-    const int n4 = vec ? r.n / 4 : 0;
+    const int n4 = vec ? n / 4 : 0;
 #pragma unroll 4
     for (int i = tid; i < n4; i += THREADS) {
         const float4 v = __ldcs(reinterpret_cast<const float4*>(src) + i);
         reinterpret_cast<float4*>(part_of_row)[i] = make_float4(take(v.x), take(v.y), take(v.z), take(v.w));
     }
 #pragma unroll 4
-    for (int i = 4 * n4 + tid; i < r.n; i += THREADS) part_of_row[i] = take(src[i]);
+    for (int i = 4 * n4 + tid; i < n; i += THREADS) part_of_row[i] = take(src[i]);
+    for (int i = n + tid; i < r.padded; i += THREADS) part_of_row[i] = -INFINITY;
     auto reduce = [&](int width) {
         for (int o = width / 2; o > 0; o >>= 1) {
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -317,6 +429,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
     reduce(32);
     if (lane == 0) { sh.warp_max[warp] = m; sh.warp_min[warp] = lowest; }
     if (tid < 16) sh.power[tid] = exp2((double)tid / 16);
+    if (cuts) clear(sh);
     __syncthreads();
     m = sh.warp_max[lane % WARPS];
     lowest = sh.warp_min[lane % WARPS];
@@ -329,7 +442,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
     if (m == -INFINITY || greedy) {
         if (m > -INFINITY) {   // the first place of the largest
             int at = 0x7fffffff;
-            for (int i = tid; i < r.n; i += THREADS)
+            for (int i = tid; i < r.padded; i += THREADS)
                 if (r.x[i] == m) { at = r.first + i; break; }
             at = __reduce_min_sync(0xffffffffu, at);
             if (lane == 0 && at < 0x7fffffff) atomicMin(&cl.map_shared_rank(&sh, 0)->at, at);
@@ -339,36 +452,34 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
         return;
     }
     if (m == INFINITY) {   // the infinite ones share the mass: as logits of 0 among -infinity
-        for (int i = tid; i < r.n; i += THREADS) part_of_row[i] = r.x[i] == INFINITY ? 0.f : -INFINITY;
+        for (int i = tid; i < r.padded; i += THREADS) part_of_row[i] = r.x[i] == INFINITY ? 0.f : -INFINITY;
         m = lowest = 0.f;
         __syncthreads();
     }
     r.max = m;
     r.min = lowest;
     r.top = m;
-    r.rate = 1.4426950408889634074 / (double)t;
+    r.fresh = true;
+    r.rate = rate;
     r.power = sh.power;
-    r.nothing = fmaxf((float)(r.top - 1000.0 / r.rate), -3.4028235e38f);
-    r.tau = key_of(-INFINITY) + 1;
-    r.last = 0x7fffffff;
+    r.nothing = fmaxf((float)(r.top - (1000.0 * 0.69314718055994530942) * (double)t), -3.4028235e38f);   // 2^-1000
+    r.tau = -3.4028235e38f;   // everything above -infinity
+    r.last = ALL;
     if (mp > 0.f) {
-        const float least = fminf(m, __double2float_ru((double)m + (double)t * log((double)fminf(mp, 1.f))) + 0.f);
-        r.tau = max(r.tau, key_of(least));
-        r.min = fmaxf(r.min, least);
+        r.tau = fmaxf(r.tau, fminf(m, __double2float_ru((double)m + (double)t * log((double)fminf(mp, 1.f))) + 0.f));
+        r.min = fmaxf(r.min, r.tau);
     }
-    if (k > 0 && k < vocab) cut<false>(cl, sh, r, k, 0.0);
-    if (p < 1.f) cut<true>(cl, sh, r, 0, p);
-    const bool all = r.tau == key_of(-INFINITY) + 1 && r.last == 0x7fffffff;
+    if (k > 0 && k < vocab && cut<false>(cl, sh, r, k, p, u[row], token + row)) return;
+    if (p < 1.f) cut<true>(cl, sh, r, 0, fmaxf(p, 1e-30f), 0.0, nullptr);   // rank 0 always stays
 
     // the draw: sums of blocks of 128 logits, the CTA in which u falls, the block, the logit
-    auto kept_weight = [&](int i, float x) { return all || kept(r, key_of(x), i) ? weight(r, x) : 0.0; };
-    auto lane_weights = [&](int block, double (&w)[4]) {   // this lane's 4 of a block; past the end: 0
+    auto lane_weights = [&](int block, double (&w)[4]) {   // this lane's 4 of a block
         const int i = block * BLOCK + 4 * lane;
         const float4 v = *reinterpret_cast<const float4*>(r.x + i);
-        w[0] = i < r.n ? kept_weight(i, v.x) : 0.0;
-        w[1] = i + 1 < r.n ? kept_weight(i + 1, v.y) : 0.0;
-        w[2] = i + 2 < r.n ? kept_weight(i + 2, v.z) : 0.0;
-        w[3] = i + 3 < r.n ? kept_weight(i + 3, v.w) : 0.0;
+        w[0] = kept(r, v.x, i) ? weight(r, v.x) : 0.0;
+        w[1] = kept(r, v.y, i + 1) ? weight(r, v.y) : 0.0;
+        w[2] = kept(r, v.z, i + 2) ? weight(r, v.z) : 0.0;
+        w[3] = kept(r, v.w, i + 3) ? weight(r, v.w) : 0.0;
     };
     auto scan = [&](double v) {   // inclusive, over the warp
 #pragma unroll
@@ -388,7 +499,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
         if (at > 0 && at < 32) ahead += x;
         return at;
     };
-    const int blocks = (r.n + BLOCK - 1) / BLOCK;
+    const int blocks = r.padded / BLOCK;
     for (int b = warp; b < blocks; b += WARPS) {
         double w[4];
         lane_weights(b, w);
@@ -417,8 +528,9 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
     const int owner = first_over(of_cta, cta_any, ahead, target);
     if (owner >= ranks) {   // u >= 1, or the sums' last bits: the last kept token that weighs anything
         int last = -1;
-        for (int i = tid; i < r.n; i += THREADS)
-            if (kept(r, key_of(r.x[i]), i) && weight(r, r.x[i]) > 0.0) last = r.first + i;
+        for_kept(r, [&](float x, int i) {
+            if (weight(r, x) > 0.0) last = max(last, r.first + i);
+        });
         last = __reduce_max_sync(0xffffffffu, last);
         __syncthreads();
         if (tid == 0) sh.last = -1;
