@@ -255,7 +255,8 @@ typedef struct {
     const int32_t* token_start;   /* device, [n_seqs + 1], ascending; NULL: one token per sequence */
     size_t n_seqs, n_tokens;      /* n_tokens: rows of the token arrays */
     size_t max_seq_len;           /* host bound of seq_len; 0: table_width * page_size */
-    size_t max_new;               /* host bound of a sequence's new tokens; 0: 1 without token_start, else n_tokens */
+    size_t max_new;               /* host bound of a sequence's new tokens; 0: 1 without token_start, else n_tokens.
+                                     The attention takes at most 65535, and works and reserves space for that many. */
 } lcu_kv_batch;
 
 /* Appends the step's keys and values, rotating q and k by their positions on the way
@@ -289,10 +290,10 @@ size_t lcu_attention_paged_workspace(const lcu_kv_pages* pages, const lcu_kv_bat
 /* One token per row of logits [rows][vocab], rows ld floats apart, vocab <= 262144. Per-row
  * device arrays; a NULL one means 1, off, off, off. With w_i = exp((x_i - max x) / temperature)
  * and ranks by falling logit, ties by rising index, a row keeps the ranks that pass all of
- *   rank < top_k (<= 0: off), w_i >= min_p (<= 0: off), and then
+ *   rank < top_k (<= 0: off), w_i >= min_p (<= 0: off; over 1 counts as 1), and then
  *   the mass of the ranks before it < top_p * the mass so kept (>= 1: off; rank 0 always stays),
  * and draws the first index at which the running mass of the kept ones, by rising index,
- * exceeds u * their mass (u in [0, 1); u >= 1 gives the last kept index). temperature <= 0 or NaN takes
+ * exceeds u * their mass (u in [0, 1); u >= 1 or NaN gives the last kept index). temperature <= 0 or NaN takes
  * the largest logit, the lowest index among equals. NaN logits count as -infinity; a row that
  * has nothing above -infinity gives -1. Masses are summed in 64 bits and do not depend on
  * the order in which the GPU runs. */

@@ -304,7 +304,10 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 
         // ---- S^T = K Q^T, 32 keys for each of q's fragments
         uint32_t kw[4][D / 32];
-        float a[NT][2][4];   // [.][16 keys]: (key g, rows 2t, 2t + 1), (key g + 8, the same)
+        // [.][16 keys]: (key g, rows 2t, 2t + 1), (key g + 8, the same). An MMA truncates its sum, so the products with q's lo
+        // halves, and the second half of 256 channels, add up apart: as many truncations of a large sum less.
+        constexpr int HALVES = D == 256 ? 2 : 1;
+        float a[NT][2][4], a_hi[HALVES][NT][2][4], a_lo[NT][2][4];
 #pragma unroll
         for (int n = 0; n < 4; n++) {
             const uint8_t* at = st + k_at + n * 8 * S::ROW;
@@ -323,7 +326,11 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int x = 0; x < 8; x++) a[nt][x >> 2][x & 3] = 0.f;
+            for (int x = 0; x < 8; x++) {
+                a_lo[nt][x >> 2][x & 3] = 0.f;
+#pragma unroll
+                for (int h = 0; h < HALVES; h++) a_hi[h][nt][x >> 2][x & 3] = 0.f;
+            }
         Scale pair[4][D == 256 ? 2 : 1];           // factors of two groups
 #pragma unroll
         for (int n = 0; n < 4; n++) {
@@ -363,8 +370,8 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
                         const uint32_t ka[4] = {h[2 * u], h8[2 * u], h[2 * u + 1], h8[2 * u + 1]};
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
-                            mma(a[nt][kb], ka, f[nt][u].x, f[nt][u].y);
-                            if (!PACK) mma(a[nt][kb], ka, f[nt][u].z, f[nt][u].w);
+                            mma(a_hi[wi * HALVES / (D / 32)][nt][kb], ka, f[nt][u].x, f[nt][u].y);
+                            if (!PACK) mma(a_lo[nt][kb], ka, f[nt][u].z, f[nt][u].w);
                         }
                     }
                 }
@@ -403,6 +410,12 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
             poison = __reduce_or_sync(0xffffffffu, poison);
         }
 
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int x = 0; x < 8; x++)
+                a[nt][x >> 2][x & 3] = a_hi[0][nt][x >> 2][x & 3] + (HALVES == 2 ? a_hi[HALVES - 1][nt][x >> 2][x & 3] : 0.f) +
+                                       (PACK ? 0.f : a_lo[nt][x >> 2][x & 3]);
         if (PACK) {   // hi + lo columns
 #pragma unroll
             for (int x = 0; x < 8; x++) a[0][x >> 2][x & 3] += __shfl_xor_sync(0xffffffffu, a[0][x >> 2][x & 3], 2);
@@ -622,7 +635,7 @@ __global__ void __launch_bounds__(THREADS) k_attn_paged_join(float* __restrict__
 
 lancius_error bad(lancius_error e) { lancius_set_error(e); return e; }
 
-int row_blocks(int rows) { return rows > 8 ? (rows + 15) / 16 : 1; }
+size_t row_blocks(int rows) { return rows > 8 ? ((size_t)rows + 15) / 16 : 1; }
 
 template <int D>
 int resident(int rows) { return rows <= 8 ? Shape<D, 8>::RESIDENT : Shape<D, 16>::RESIDENT; }
@@ -650,8 +663,10 @@ size_t part_rows(const KvBatchDev& b, size_t hq, Split sp) { return (size_t)b.n_
 lancius_error check_call(const lcu_kv_pages* pages, const lcu_kv_batch* batch, size_t n_q_heads, KvPagesDev* p, KvBatchDev* b) {
     lancius_error e = lcu_kv_describe(pages, batch, p, b);
     if (e != LANCIUS_ERROR_OK) return e;
-    const size_t rows = n_q_heads / pages->n_heads * b->max_new;
-    if (n_q_heads > 65535 || n_q_heads % pages->n_heads || b->max_new > 65535 || rows > (size_t)INT32_MAX / 2)
+    if (n_q_heads > 65535 || n_q_heads % pages->n_heads || b->max_new > 65535) return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
+    const Split sp = plan(*p, *b, (int)pages->head_dim, (int)(n_q_heads / pages->n_heads));
+    if ((size_t)sp.splits * row_blocks((int)(n_q_heads / pages->n_heads) * b->max_new) > (size_t)INT32_MAX ||
+        part_rows(*b, n_q_heads, sp) > (size_t)1 << 40)
         return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
     return LANCIUS_ERROR_OK;
 }
@@ -660,7 +675,8 @@ template <int D, int ROWS>
 lancius_error launch(float* out, const float* q, size_t q_ld, int hq, const KvPagesDev& p, const KvBatchDev& b, Split sp,
                      float* part_o, float2* part_ml, cudaStream_t st) {
     using S = Shape<D, ROWS>;
-    cudaError_t ce = cudaFuncSetAttribute(k_attn_paged<D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    static std::atomic<unsigned long long> allowed{0};   // devices on which the kernel may use its shared memory
+    cudaError_t ce = lcu_allow_smem(allowed, k_attn_paged<D, ROWS>, S::SMEM);
     if (ce != cudaSuccess) return lcu_check_cuda(ce);
     const dim3 grid((unsigned)(sp.splits * row_blocks(hq / p.heads * b.max_new)), (unsigned)p.heads, (unsigned)b.n_seqs);
     k_attn_paged<D, ROWS><<<grid, THREADS, S::SMEM, st>>>(out, q, q_ld, hq, p, b, (float)(1.4426950408889634 / sqrt((double)D)), sp,

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <stddef.h>
+#include <atomic>
 #include "lancius_cuda.h"
 
 #define LCU_SMS 148   // B200: 2 dies x 74 SMs
@@ -38,6 +39,19 @@ __device__ __forceinline__ float lcu_apply_epi(float v, int epi) {
     if (epi == LCU_EPI_RELU) return v > 0.f ? v : 0.f;
     if (epi == LCU_EPI_GELU) return lcu_gelu_f(v);
     return v;
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device; `done` remembers the devices (a bit each).
+template <typename Kernel>
+static inline cudaError_t lcu_allow_smem(std::atomic<unsigned long long>& done, Kernel kernel, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 // Launch-count bookkeeping used by the executor and the per-op API.

@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
     r.nothing = fmaxf((float)(r.top - (1000.0 * 0.69314718055994530942) * (double)t), -3.4028235e38f);   // 2^-1000
     r.tau = -3.4028235e38f;   // everything above -infinity
     r.last = ALL;
-    if (mp > 0.f) {
+    if (mp > 0.f && t < INFINITY) {
         r.tau = fmaxf(r.tau, fminf(m, __double2float_ru((double)m + (double)t * log((double)fminf(mp, 1.f))) + 0.f));
         r.min = fmaxf(r.min, r.tau);
     }
@@ -588,7 +588,8 @@ extern "C" lancius_error lcu_sample(int32_t* token, const float* logits, size_t 
     if (!vocab || vocab > MAX_VOCAB || ld < vocab || rows > (size_t)INT32_MAX / MAX_CLUSTER) return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
     const int c = cluster_of(rows, vocab);
     const size_t part = ((vocab + c - 1) / c + 3) / 4 * 4, space = (part + BLOCK - 1) / BLOCK * BLOCK;   // whole blocks are read
-    cudaError_t ce = cudaFuncSetAttribute(k_sample, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(MAX_VOCAB / MAX_CLUSTER * sizeof(float)));
+    static std::atomic<unsigned long long> allowed{0};
+    cudaError_t ce = lcu_allow_smem(allowed, k_sample, (int)(MAX_VOCAB / MAX_CLUSTER * sizeof(float)));
     if (ce != cudaSuccess) return lcu_check_cuda(ce);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at[1];

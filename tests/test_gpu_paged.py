@@ -463,6 +463,25 @@ def test_sample_follows_the_distribution(lib):
     assert np.all(np.abs(got - n * w / w.sum()) <= 1.0)
 
 
+@pytest.mark.parametrize("vocab", [5000, 40000, 262144])
+def test_sample_many_equal_logits(lib, vocab):
+    """More equal logits at the cut than a list holds; rows that are mostly masked with the type's lowest value."""
+    rng = np.random.default_rng(vocab)
+    x = np.zeros((5, vocab), np.float32)
+    x[1, ::3] = 2.5
+    x[2] = np.round(rng.standard_normal(vocab))
+    x[3] = np.float32(-3.4028235e38)
+    some = rng.choice(vocab, 2000, replace=False)
+    x[3, some] = rng.standard_normal(2000)
+    x[4] = -np.inf
+    x[4, some] = np.round(rng.standard_normal(2000) * 4) / 4
+    for u in (0.0, 0.31, 0.77, 0.999):
+        uu = np.full(5, u, np.float32)
+        for kw in (dict(top_k=1500), dict(top_k=700, top_p=0.37), dict(top_p=0.37), dict(top_p=0.9999), dict(top_k=300, min_p=0.5),
+                   dict(min_p=0.01, top_p=0.63, temperature=0.4)):
+            check_sample(sample(lib, x, uu, **kw), x, uu, **kw)
+
+
 # ---- together ----------------------------------------------------------------------------------------------------
 
 def model(lib, seed, hq, heads, dim, vocab):
@@ -553,6 +572,68 @@ def test_decode_loop_matches_prompt_pass(lib, dim, page):
     for s in range(seqs):
         got = bufs[4].view(seqs, n)[s].cpu().numpy()
         check_sample(got, logits[s], u[:, s].cpu().numpy())
+
+
+def test_cache_past_32_bit_offsets(lib):
+    """Rows that start more than 2^32 bytes into the cache."""
+    dim, page, heads = 256, 4096, 1
+    total = 2 ** 32 // (page * dim // 2) + 40   # pages; a page holds 512 KB of codes
+    mk = lambda w: torch.empty((total, heads, page, w), dtype=torch.uint8, device="cuda")
+    c = Cache([5000, 300], heads, dim, page, seed=1)   # its table only
+    c.kc, c.vc, c.ks, c.vs = mk(dim // 2), mk(dim // 2), mk(dim // 16), mk(dim // 16)
+    c.table_np = np.array([[total - 1, total - 3], [total - 2, 0]], np.int32)
+    c.table = i32(c.table_np)
+    c.pages = L.KvPages(ptr(c.kc), ptr(c.vc), ptr(c.ks), ptr(c.vs), total, page, heads, dim, 1.0, 1.0)
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((5300, 3, dim)).astype(np.float32)
+    b = c.batch([5000, 300], [0, 5000, 5300])
+    q = append(lib, c, b, x.reshape(5300, -1), 1)
+    ko, vo = torch.zeros((5300, 1, dim), device="cuda"), torch.zeros((5300, 1, dim), device="cuda")
+    assert lib.lcu_kv_read_paged(ptr(ko), ptr(vo), c.pages, b, None) == 0
+    b = c.batch([5000, 300])
+    out = attend(lib, c, b, q[[4999, 5299]], 1)
+    assert lib.lcu_check_stream(None) == 0
+    at = 0
+    for s, n in enumerate((5000, 300)):
+        k, v = ko[at:at + n].double().cpu().numpy(), vo[at:at + n].double().cpu().numpy()
+        assert np.array_equal(v[:, 0], kvref.values(*kvref.quantise(x[at:at + n, 2])))
+        row = q[[4999, 5299]][s].reshape(1, 1, dim)
+        ref, size = kvref.attention(row, k, v, [n])
+        assert np.max(np.abs(out[s] - ref.reshape(-1))) <= tolerance(size, dim, np.abs(v).max(), n)
+        at += n
+
+
+def test_captured_split_attention_follows_lengths(lib):
+    """One captured call, replayed with other lengths (chunks come and go) and other page tables."""
+    c = Cache([9000, 3000], 2, 128, 16, seed=2)
+    fill_random(c, 21)
+    q = np.random.default_rng(3).standard_normal((2, 4, 128)).astype(np.float32)
+    t = torch.from_numpy(q.reshape(2, -1)).cuda()
+    out = torch.zeros((2, 4 * 128), device="cuda")
+    lens = i32([9000, 3000])
+    b = L.KvBatch(ptr(c.table), c.table.shape[1], ptr(lens), None, 2, 2, 9000, 1)
+    need = lib.lcu_attention_paged_workspace(c.pages, b, 4)
+    assert need > 0
+    space = torch.full((need,), 0xff, dtype=torch.uint8, device="cuda")
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert lib.lcu_attention_paged(ptr(out), ptr(t), 512, 4, c.pages, b, ptr(space), need, side.cuda_stream) == 0
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            assert lib.lcu_attention_paged(ptr(out), ptr(t), 512, 4, c.pages, b, ptr(space), need, side.cuda_stream) == 0
+        for n in ([9000, 3000], [1, 2999], [0, 17], [8999, 128]):
+            lens.copy_(i32(n))
+            out.fill_(7.0)
+            g.replay()
+            side.synchronize()
+            got = out.view(2, 4, 128).cpu().numpy()
+            for s in range(2):
+                k, v = c.kv(s, n[s])
+                ref, size = kvref.attention(q[s:s + 1], k, v, [n[s]])
+                tol = tolerance(size, 128, np.abs(v).max() if n[s] else 1.0, n[s])
+                assert np.max(np.abs(got[s] - ref[0])) <= tol
+    assert lib.lcu_check_stream(side.cuda_stream) == 0
 
 
 def test_two_streams_at_once(lib):

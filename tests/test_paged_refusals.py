@@ -73,6 +73,10 @@ def test_attention_refused():
     assert lib.lcu_attention_paged(AT, AT, 256, 3, p, b, AT, 1 << 30, None) == SHAPE
     assert lib.lcu_attention_paged(AT, AT, 256, 4, None, b, AT, 1 << 30, None) == NULL
     assert lib.lcu_attention_paged(AT, AT, 256, 4, p, None, AT, 1 << 30, None) == NULL
+    many = batch(token_start=AT, n_tokens=70000)   # max_new 0: up to n_tokens per sequence
+    assert lib.lcu_attention_paged(AT, AT, 256, 4, p, many, AT, 1 << 40, None) == SHAPE
+    assert lib.lcu_attention_paged_workspace(p, many, 4) == 0
+    assert lib.lcu_attention_paged(AT, AT, 256, 4, pages(n_pages=1 << 28), b, AT, 1 << 30, None) == SHAPE   # rows past 32 bits
 
 
 def test_nothing_to_do():
