@@ -56,7 +56,7 @@ struct Row {
     int padded, first;  // its length and the index of its first token
     float max, min;     // of the row, min over the finite ones
     double top, rate;   // max, log2(e) / t
-    float nothing;      // weights are 0 below this logit
+    float nothing;      // weights fall no further below this logit
     const double* power;   // 2^(j/16), in shared memory
     bool fresh;         // the histogram is cleared
     float tau;          // kept: logit > tau, or logit == tau and index <= last
@@ -79,13 +79,10 @@ __device__ __forceinline__ void for_kept(const Row& r, Use use) {
         if (kept(r, v.w, 4 * j + 3)) use(v.w, 4 * j + 3);
     }
 }
-// exp((x - max) / t) as 2^z, z = n / 16 + f, |f| <= 1/32: a table of 2^(j/16) times the Taylor series of 2^f to f^6
+// 2^z, z = n / 16 + f, |f| <= 1/32: a table of 2^(j/16) times the Taylor series of 2^f to f^6
 // (table-driven exponential, Tang 1989); the series' remainder is 5e-16. 13 FP64 instructions, where the library's
-// exp and a division took 124 of all kinds. Below 2^-1000 the
-// weight is 0.
-__device__ __forceinline__ double weight(const Row& r, float x) {
-    if (!(x >= r.nothing)) return 0.0;
-    const double z = ((double)x - r.top) * r.rate;
+// exp and a division took 124 of all kinds. For z > -1022.
+__device__ __forceinline__ double power_of_two(double z, const double* power) {
     constexpr double MAGIC = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the rounded integer
     const double k = fma(z, 16.0, MAGIC);
     const int n = __double2loint(k);
@@ -96,9 +93,15 @@ __device__ __forceinline__ double weight(const Row& r, float x) {
     p = fma(p, f, 5.5504108664821579953e-2);
     p = fma(p, f, 2.4022650695910071233e-1);
     p = fma(p, f, 6.9314718055994530942e-1);
-    p = fma(p, f, 1.0) * r.power[n & 15];
+    p = fma(p, f, 1.0) * power[n & 15];
     return __hiloint2double(__double2hiint(p) + ((n >> 4) << 20), __double2loint(p));
 }
+// Without branches: logits below `nothing` weigh as much as that one, 2^-1000, and only -infinity weighs 0.
+__device__ __forceinline__ double weight_of(float x, double top, float nothing, double rate, const double* power) {
+    const double w = power_of_two(((double)fmaxf(x, nothing) - top) * rate, power);
+    return x > -INFINITY ? w : 0.0;
+}
+__device__ __forceinline__ double weight(const Row& r, float x) { return weight_of(x, r.top, r.nothing, r.rate, r.power); }
 __device__ __forceinline__ u64 fixed_weight(const Row& r, float x) {   // times 2^44, rounded
     return (u64)__double_as_longlong(fma(weight(r, x), FIXED, 4503599627370496.0)) & 0xfffffffffffffull;
 }
@@ -386,6 +389,54 @@ __device__ bool cut(cg::cluster_group& cl, Shared& sh, Row& r, int k, double p, 
     }
 }
 
+__device__ __forceinline__ double scan(double v) {   // inclusive, over the warp
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+    }
+    return v;
+}
+// v: inclusive sums by lane of what each lane has, if any; the first lane that has some and whose sum, behind `ahead`,
+// passes the target (32: none); ahead moves to its start. A sum's last bits depend on its order, so a lane without
+// weight may seem to pass.
+__device__ __forceinline__ int first_over(double v, bool any, double& ahead, double target) {
+    const unsigned over = __ballot_sync(0xffffffffu, any && ahead + v > target);
+    const int at = over ? __ffs(over) - 1 : 32;
+    const double x = __shfl_sync(0xffffffffu, v, max(min(at, 31) - 1, 0));
+    if (at > 0 && at < 32) ahead += x;
+    return at;
+}
+// Where no lane passes, again for the last bits, the last that has some.
+__device__ __forceinline__ int or_last(int at, bool any) {
+    const unsigned some = __ballot_sync(0xffffffffu, any);
+    return at < 32 ? at : 31 - __clz(some);
+}
+// One warp draws within its CTA: mine, the inclusive sums by lane of per neighbouring blocks each; block_mass, the blocks'
+// sums; lane_weights(block, w), the weights of the lane's 4 logits of a block. Returns the index in the CTA's part.
+template <typename Weights>
+__device__ __forceinline__ int draw_in_part(double mine, bool mine_any, int per, int blocks, const double* block_mass, double ahead,
+                                            double target, Weights lane_weights) {
+    const int lane = threadIdx.x & 31;
+    int at = or_last(first_over(mine, mine_any, ahead, target), mine_any);
+    const int b0 = at * per, n = min(per, blocks - b0);   // per <= 8 blocks
+    const double of_block = lane < n ? block_mass[b0 + lane] : 0.0;
+    const int block = b0 + or_last(first_over(scan(of_block), of_block > 0.0, ahead, target), of_block > 0.0);
+    double w[4];
+    lane_weights(block, w);
+    const double four = (w[0] + w[1]) + (w[2] + w[3]);
+    at = or_last(first_over(scan(four), four > 0.0, ahead, target), four > 0.0);
+    int drawn = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (w[j] > 0.0 && !(ahead > target)) {
+            drawn = j;
+            ahead += w[j];
+        }
+    return __shfl_sync(0xffffffffu, block * BLOCK + 4 * lane + drawn, at);
+}
+
 __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ token, const float* __restrict__ logits, size_t ld, int vocab,
                                                     int part, int vec, const float* temperature, const int32_t* top_k,
                                                     const float* top_p, const float* min_p, const float* u) {
@@ -476,28 +527,13 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
     auto lane_weights = [&](int block, double (&w)[4]) {   // this lane's 4 of a block
         const int i = block * BLOCK + 4 * lane;
         const float4 v = *reinterpret_cast<const float4*>(r.x + i);
-        w[0] = kept(r, v.x, i) ? weight(r, v.x) : 0.0;
-        w[1] = kept(r, v.y, i + 1) ? weight(r, v.y) : 0.0;
-        w[2] = kept(r, v.z, i + 2) ? weight(r, v.z) : 0.0;
-        w[3] = kept(r, v.w, i + 3) ? weight(r, v.w) : 0.0;
-    };
-    auto scan = [&](double v) {   // inclusive, over the warp
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double x = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += x;
-        }
-        return v;
-    };
-    // v: inclusive sums by lane of what each lane has, if any; the first lane that has some and whose sum, behind `ahead`,
-    // passes the target (32: none); ahead moves to its start. A sum's last bits depend on its order, so a lane without
-    // weight may seem to pass.
-    auto first_over = [&](double v, bool any, double& ahead, double target) {
-        const unsigned over = __ballot_sync(0xffffffffu, any && ahead + v > target);
-        const int at = over ? __ffs(over) - 1 : 32;
-        const double x = __shfl_sync(0xffffffffu, v, max(min(at, 31) - 1, 0));
-        if (at > 0 && at < 32) ahead += x;
-        return at;
+        const bool k0 = kept(r, v.x, i), k1 = kept(r, v.y, i + 1), k2 = kept(r, v.z, i + 2), k3 = kept(r, v.w, i + 3);
+        w[0] = w[1] = w[2] = w[3] = 0.0;
+        if (!__any_sync(0xffffffffu, k0 || k1 || k2 || k3)) return;
+        w[0] = weight(r, k0 ? v.x : -INFINITY);
+        w[1] = weight(r, k1 ? v.y : -INFINITY);
+        w[2] = weight(r, k2 ? v.z : -INFINITY);
+        w[3] = weight(r, k3 ? v.w : -INFINITY);
     };
     const int blocks = r.padded / BLOCK;
     for (int b = warp; b < blocks; b += WARPS) {
@@ -541,28 +577,151 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
         return;
     }
     if (owner == rank && warp == 0) {
-        // where no lane passes, again for the last bits, the last that has some is taken
-        auto or_last = [&](int at, bool any) {
-            const unsigned some = __ballot_sync(0xffffffffu, any);
-            return at < 32 ? at : 31 - __clz(some);
-        };
-        int at = or_last(first_over(mine, mine_any, ahead, target), mine_any);
-        const int b0 = at * per, n = min(per, blocks - b0);   // per <= 8 blocks
-        const double of_block = lane < n ? sh.block_mass[b0 + lane] : 0.0;
-        const int block = b0 + or_last(first_over(scan(of_block), of_block > 0.0, ahead, target), of_block > 0.0);
-        double w[4];
-        lane_weights(block, w);
-        const double four = (w[0] + w[1]) + (w[2] + w[3]);
-        at = or_last(first_over(scan(four), four > 0.0, ahead, target), four > 0.0);
-        if (lane == at) {
-            int drawn = -1;
-            for (int j = 0; j < 4; j++)
-                if (w[j] > 0.0) {
-                    drawn = j;
-                    ahead += w[j];
-                    if (ahead > target) break;
-                }
-            token[row] = r.first + block * BLOCK + 4 * lane + drawn;
+        const int at = draw_in_part(mine, mine_any, per, blocks, sh.block_mass, ahead, target, lane_weights);
+        if (lane == 0) token[row] = r.first + at;
+    }
+    cl.sync();   // nobody leaves while its shared memory is read
+}
+
+// Without filters: one pass. Each warp takes blocks of 128 logits, whose weights are summed relative to the block's own
+// maximum; the sums are brought to the row's maximum when that is known, and the drawn block's logits are read again.
+// Nothing of a row stays in shared memory but a maximum and a sum per block, so twice as many CTAs run as above.
+constexpr int OPEN_THREADS = 256, OPEN_WARPS = OPEN_THREADS / 32;
+
+__global__ void __launch_bounds__(OPEN_THREADS, 4) k_sample_open(int32_t* __restrict__ token, const float* __restrict__ logits,
+                                                                 size_t ld, int vocab, int part, int vec, const float* temperature,
+                                                                 const float* u) {
+    __shared__ double block_mass[MAX_BLOCKS], power[16], mass_here;
+    __shared__ float block_max[MAX_BLOCKS], warp_max[OPEN_WARPS], max_here;
+    __shared__ int first_here;
+    cg::cluster_group cl = cg::this_cluster();
+    const int ranks = cl.num_blocks(), rank = cl.block_rank(), row = blockIdx.x / ranks, first = rank * part;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int n = max(0, min(part, vocab - first)), blocks = (n + BLOCK - 1) / BLOCK;
+    const float* src = logits + (size_t)row * ld + first;
+    const float t = temperature ? temperature[row] : 1.f;
+    const double rate = 1.4426950408889634074 / (double)t;
+    const bool greedy = !(t > 0.f);
+    if (tid < 16) power[tid] = exp2((double)tid / 16);
+    if (tid == 0) first_here = ALL;
+    __syncthreads();
+    auto fetch = [&](int block, float (&x)[4], bool in_order) {   // a block's logits; in order: 4 neighbours a lane
+        const int i = block * BLOCK + 4 * lane;
+        if (vec && i + 3 < n) {
+            const float4 v = *reinterpret_cast<const float4*>(src + i);
+            x[0] = clean(v.x); x[1] = clean(v.y); x[2] = clean(v.z); x[3] = clean(v.w);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int k = vec || in_order ? i + j : block * BLOCK + 32 * j + lane;
+                x[j] = k < n ? clean(src[k]) : -INFINITY;
+            }
+        }
+    };
+    const float reach = 693.f * t;   // 2^-1000
+    auto lane_weights = [&](const float (&x)[4], float top, double (&w)[4]) {   // relative to top
+        if (top == INFINITY) {       // the infinite ones share the mass
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[j] = x[j] == INFINITY ? 1.0 : 0.0;
+        } else {
+            const float nothing = fmaxf(top - reach, -3.4028235e38f);
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[j] = weight_of(x[j], top, nothing, rate, power);
+        }
+    };
+    constexpr int AHEAD = 2;   // blocks of a warp in flight
+    float x[AHEAD][4], m = -INFINITY;
+#pragma unroll
+    for (int a = 0; a < AHEAD; a++)
+        if (warp + a * OPEN_WARPS < blocks) fetch(warp + a * OPEN_WARPS, x[a], false);
+    for (int b0 = warp; b0 < blocks; b0 += AHEAD * OPEN_WARPS) {
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            const int b = b0 + a * OPEN_WARPS;
+            if (b >= blocks) break;
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] = x[a][j];
+            if (b + AHEAD * OPEN_WARPS < blocks) fetch(b + AHEAD * OPEN_WARPS, x[a], false);
+            float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            double v = 0.0;
+            if (!greedy && top > -INFINITY) {
+                double w[4];
+                lane_weights(y, top, w);
+                v = (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            }
+            if (lane == 0) { block_max[b] = top; block_mass[b] = v; }
+            m = fmaxf(m, top);
+        }
+    }
+    if (lane == 0) warp_max[warp] = m;
+    __syncthreads();
+    m = warp_max[lane % OPEN_WARPS];
+#pragma unroll
+    for (int o = OPEN_WARPS / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (tid == 0) max_here = m;
+    cl.sync();
+    m = *cl.map_shared_rank(&max_here, lane % ranks);
+#pragma unroll
+    for (int o = MAX_CLUSTER / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    // of this CTA's blocks: per neighbours a lane of the first warp
+    double mine = 0.0;
+    bool mine_any = false;
+    const int per = (blocks + 31) / 32;
+    if (warp == 0) {
+        int at = ALL;   // the first block that holds the row's maximum
+        for (int k = 0; k < per; k++) {
+            const int b = lane * per + k;
+            if (b >= blocks) break;
+            const float top = block_max[b];
+            if (top == m) at = min(at, b);
+            double v = 0.0;
+            if (!greedy && m == INFINITY) v = top == m ? block_mass[b] : 0.0;
+            else if (!greedy) v = block_mass[b] * weight_of(top, m, fmaxf(m - reach, -3.4028235e38f), rate, power);
+            block_mass[b] = v;
+            mine += v;
+        }
+        mine_any = mine > 0.0;
+        mine = scan(mine);
+        if (lane == 31) mass_here = mine;
+        if (greedy && m > -INFINITY) {
+            at = __reduce_min_sync(0xffffffffu, at);
+            if (at < ALL) {
+                float y[4];
+                fetch(at, y, true);
+                const int mark = y[0] == m ? 0 : y[1] == m ? 1 : y[2] == m ? 2 : y[3] == m ? 3 : ALL;
+                const unsigned hit = __ballot_sync(0xffffffffu, mark < ALL);
+                const int l = __ffs(hit) - 1;
+                const int j = __shfl_sync(0xffffffffu, mark, l);
+                if (lane == 0) first_here = first + at * BLOCK + 4 * l + j;
+            }
+        }
+    }
+    cl.sync();
+    if (warp == 0) {
+        if (m == -INFINITY || greedy) {
+            const int at = __reduce_min_sync(0xffffffffu, *cl.map_shared_rank(&first_here, lane % ranks));
+            if (rank == 0 && lane == 0) token[row] = m == -INFINITY ? -1 : at;
+        } else {
+            double of_cta = lane < ranks ? *cl.map_shared_rank(&mass_here, lane % ranks) : 0.0;
+            const bool cta_any = of_cta > 0.0;
+            of_cta = scan(of_cta);
+            const double total = __shfl_sync(0xffffffffu, of_cta, 31), target = (double)u[row] * total;
+            double ahead = 0.0;
+            // u >= 1 draws from the last that has any, and there the last
+            const int owner = or_last(first_over(of_cta, cta_any, ahead, target), cta_any);
+            if (owner == rank) {
+                const int at = draw_in_part(mine, mine_any, per, blocks, block_mass, ahead, target, [&](int block, double (&w)[4]) {
+                    float y[4];
+                    fetch(block, y, true);
+                    lane_weights(y, m, w);
+                });
+                if (lane == 0) token[row] = first + at;
+            }
         }
     }
     cl.sync();   // nobody leaves while its shared memory is read
@@ -570,11 +729,13 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
 
 lancius_error bad(lancius_error e) { lancius_set_error(e); return e; }
 
-// CTAs per row: parts of at most 16384 logits, so that two CTAs fit on an SM, and for few rows up to 8 with at least 2048
-int cluster_of(size_t rows, size_t vocab) {
+// CTAs per row. With filters parts of at most 16384 logits, so that two CTAs fit on an SM, without them of 32768; for few
+// rows up to 8 with at least 2048, as long as all CTAs run at once.
+int cluster_of(size_t rows, size_t vocab, bool open) {
+    const size_t resident = (open ? 4 : 2) * LCU_SMS, most = open ? 32768 : 16384;
     int c = 1;
-    while (c < MAX_CLUSTER && vocab > 16384 * (size_t)c) c *= 2;
-    while (c < MAX_CLUSTER && rows * c * 2 <= 2 * LCU_SMS && vocab >= 4096 * (size_t)c) c *= 2;
+    while (c < MAX_CLUSTER && vocab > most * c) c *= 2;
+    while (c < MAX_CLUSTER && rows * c * 2 <= resident && vocab >= 4096 * (size_t)c) c *= 2;
     return c;
 }
 
@@ -586,24 +747,30 @@ extern "C" lancius_error lcu_sample(int32_t* token, const float* logits, size_t 
     if (!rows) return LANCIUS_ERROR_OK;
     if (!token || !logits || !u) return bad(LANCIUS_ERROR_NULL_PTR);
     if (!vocab || vocab > MAX_VOCAB || ld < vocab || rows > (size_t)INT32_MAX / MAX_CLUSTER) return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
-    const int c = cluster_of(rows, vocab);
-    const size_t part = ((vocab + c - 1) / c + 3) / 4 * 4, space = (part + BLOCK - 1) / BLOCK * BLOCK;   // whole blocks are read
-    static std::atomic<unsigned long long> allowed{0};
-    cudaError_t ce = lcu_allow_smem(allowed, k_sample, (int)(MAX_VOCAB / MAX_CLUSTER * sizeof(float)));
-    if (ce != cudaSuccess) return lcu_check_cuda(ce);
+    const bool open = !top_k && !top_p && !min_p;
+    const int c = cluster_of(rows, vocab, open);
+    const size_t part = ((vocab + c - 1) / c + 3) / 4 * 4;
+    const int vec = (uintptr_t)logits % 16 == 0 && ld % 4 == 0;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = c;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)(rows * c));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = space * sizeof(float);
+    cfg.blockDim = dim3(open ? OPEN_THREADS : THREADS);
     cfg.stream = lcu_as_stream(stream);
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    const int vec = (uintptr_t)logits % 16 == 0 && ld % 4 == 0;
-    ce = cudaLaunchKernelEx(&cfg, k_sample, token, logits, ld, (int)vocab, (int)part, vec, temperature, top_k, top_p, min_p, u);
+    cudaError_t ce;
+    if (open) {
+        ce = cudaLaunchKernelEx(&cfg, k_sample_open, token, logits, ld, (int)vocab, (int)part, vec, temperature, u);
+    } else {
+        static std::atomic<unsigned long long> allowed{0};
+        ce = lcu_allow_smem(allowed, k_sample, (int)(MAX_VOCAB / MAX_CLUSTER * sizeof(float)));
+        if (ce != cudaSuccess) return lcu_check_cuda(ce);
+        cfg.dynamicSmemBytes = (part + BLOCK - 1) / BLOCK * BLOCK * sizeof(float);   // whole blocks are read
+        ce = cudaLaunchKernelEx(&cfg, k_sample, token, logits, ld, (int)vocab, (int)part, vec, temperature, top_k, top_p, min_p, u);
+    }
     if (ce != cudaSuccess) {
         cudaGetLastError();
         return lcu_check_cuda(ce);
