@@ -77,8 +77,8 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool v
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
@@ -544,8 +544,8 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 #pragma unroll
         for (int j = 0; j < D / 16; j += 2)
             if (!PACK || t < 2)
-            *reinterpret_cast<float4*>(at + 2 * j) = make_float4(o[r >> 1][j][r & 1], o[r >> 1][j][2 + (r & 1)],
-                                                                 o[r >> 1][j + 1][r & 1], o[r >> 1][j + 1][2 + (r & 1)]);
+                *reinterpret_cast<float4*>(at + 2 * j) = make_float4(o[r >> 1][j][r & 1], o[r >> 1][j][2 + (r & 1)],
+                                                                     o[r >> 1][j + 1][r & 1], o[r >> 1][j + 1][2 + (r & 1)]);
     }
     __syncthreads();
     for (int x = tid; x < cols * (D / 4); x += THREADS) {
@@ -663,7 +663,9 @@ size_t part_rows(const KvBatchDev& b, size_t hq, Split sp) { return (size_t)b.n_
 lancius_error check_call(const lcu_kv_pages* pages, const lcu_kv_batch* batch, size_t n_q_heads, KvPagesDev* p, KvBatchDev* b) {
     lancius_error e = lcu_kv_describe(pages, batch, p, b);
     if (e != LANCIUS_ERROR_OK) return e;
-    if (n_q_heads > 65535 || n_q_heads % pages->n_heads || b->max_new > 65535) return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
+    if (n_q_heads > 65535 || n_q_heads % pages->n_heads || b->max_new > 65535 ||
+        n_q_heads / pages->n_heads * b->max_new > (size_t)INT32_MAX / 2)
+        return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
     const Split sp = plan(*p, *b, (int)pages->head_dim, (int)(n_q_heads / pages->n_heads));
     if ((size_t)sp.splits * row_blocks((int)(n_q_heads / pages->n_heads) * b->max_new) > (size_t)INT32_MAX ||
         part_rows(*b, n_q_heads, sp) > (size_t)1 << 40)

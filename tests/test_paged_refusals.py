@@ -77,6 +77,9 @@ def test_attention_refused():
     assert lib.lcu_attention_paged(AT, AT, 256, 4, p, many, AT, 1 << 40, None) == SHAPE
     assert lib.lcu_attention_paged_workspace(p, many, 4) == 0
     assert lib.lcu_attention_paged(AT, AT, 256, 4, pages(n_pages=1 << 28), b, AT, 1 << 30, None) == SHAPE   # rows past 32 bits
+    wide = batch(token_start=AT, n_tokens=65000, max_new=65000)   # rows of one KV head past 31 bits
+    assert lib.lcu_attention_paged(AT, AT, 65000 * 64, 65000, pages(n_heads=1), wide, AT, 1 << 60, None) == SHAPE
+    assert lib.lcu_attention_paged_workspace(pages(n_heads=1), wide, 65000) == 0
 
 
 def test_nothing_to_do():
