@@ -293,8 +293,8 @@ size_t lcu_attention_paged_workspace(const lcu_kv_pages* pages, const lcu_kv_bat
  *   rank < top_k (<= 0: off), w_i >= min_p (<= 0: off; over 1 counts as 1), and then
  *   the mass of the ranks before it < top_p * the mass so kept (>= 1: off; rank 0 always stays),
  * and draws the first index at which the running mass of the kept ones, by rising index,
- * exceeds u * their mass (u in [0, 1); u >= 1 or NaN gives the last kept index). temperature <= 0 or NaN takes
- * the largest logit, the lowest index among equals. NaN logits count as -infinity; a row that
+ * exceeds u * their mass (u in [0, 1); u >= 1 or NaN gives the last kept index that has any).
+ * A weight below 2^-1000 of the largest counts as zero. temperature <= 0 or NaN takes the largest logit, the lowest index among equals. NaN logits count as -infinity; a row that
  * has nothing above -infinity gives -1. Masses are summed in 64 bits and do not depend on
  * the order in which the GPU runs. */
 lancius_error lcu_sample(int32_t* token, const float* logits, size_t ld, size_t rows, size_t vocab,

@@ -56,7 +56,7 @@ struct Row {
     int padded, first;  // its length and the index of its first token
     float max, min;     // of the row, min over the finite ones
     double top, rate;   // max, log2(e) / t
-    float nothing;      // weights fall no further below this logit
+    float nothing;      // weights are 0 below this logit
     const double* power;   // 2^(j/16), in shared memory
     bool fresh;         // the histogram is cleared
     float tau;          // kept: logit > tau, or logit == tau and index <= last
@@ -96,10 +96,10 @@ __device__ __forceinline__ double power_of_two(double z, const double* power) {
     p = fma(p, f, 1.0) * power[n & 15];
     return __hiloint2double(__double2hiint(p) + ((n >> 4) << 20), __double2loint(p));
 }
-// Without branches: logits below `nothing` weigh as much as that one, 2^-1000, and only -infinity weighs 0.
+// exp((x - top) / t) without branches; 0 below `nothing`, 2^-1000.
 __device__ __forceinline__ double weight_of(float x, double top, float nothing, double rate, const double* power) {
     const double w = power_of_two(((double)fmaxf(x, nothing) - top) * rate, power);
-    return x > -INFINITY ? w : 0.0;
+    return x >= nothing ? w : 0.0;
 }
 __device__ __forceinline__ double weight(const Row& r, float x) { return weight_of(x, r.top, r.nothing, r.rate, r.power); }
 __device__ __forceinline__ u64 fixed_weight(const Row& r, float x) {   // times 2^44, rounded
@@ -293,7 +293,7 @@ __device__ void finish_small(cg::cluster_group& cl, Shared& sh, const Row& r, in
         for (int j = 0; j < n; j++)
             if ((uint32_t)sh.list[j] >= (uint32_t)me) upto += sh.list_mass[j];   // indices up to this one
         if (w && (double)upto > target) atomicMin(&sh.at, index);
-        if (w || rank == 0) atomicMax(&sh.last, index);
+        if (of_key((uint32_t)(me >> 32)) >= r.nothing) atomicMax(&sh.last, index);
     }
     __syncthreads();
     if (tid == 0) *token = sh.at < 0x7fffffff ? sh.at : sh.last;
@@ -513,7 +513,8 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
     r.fresh = true;
     r.rate = rate;
     r.power = sh.power;
-    r.nothing = fmaxf((float)(r.top - (1000.0 * 0.69314718055994530942) * (double)t), -3.4028235e38f);   // 2^-1000
+    // 2^-1000; rounded up, so that far from zero the logits next to the largest stay within the exponent's range
+    r.nothing = fmaxf(__double2float_ru(r.top - (1000.0 * 0.69314718055994530942) * (double)t), -3.4028235e38f);
     r.tau = -3.4028235e38f;   // everything above -infinity
     r.last = ALL;
     if (mp > 0.f && t < INFINITY) {
@@ -618,13 +619,13 @@ __global__ void __launch_bounds__(OPEN_THREADS, 4) k_sample_open(int32_t* __rest
             }
         }
     };
-    const float reach = 693.f * t;   // 2^-1000
+    const float reach = 693.f * t;   // 2^-1000, rounded up where it is subtracted
     auto lane_weights = [&](const float (&x)[4], float top, double (&w)[4]) {   // relative to top
         if (top == INFINITY) {       // the infinite ones share the mass
 #pragma unroll
             for (int j = 0; j < 4; j++) w[j] = x[j] == INFINITY ? 1.0 : 0.0;
         } else {
-            const float nothing = fmaxf(top - reach, -3.4028235e38f);
+            const float nothing = fmaxf(__fsub_ru(top, reach), -3.4028235e38f);
 #pragma unroll
             for (int j = 0; j < 4; j++) w[j] = weight_of(x[j], top, nothing, rate, power);
         }
@@ -681,7 +682,7 @@ __global__ void __launch_bounds__(OPEN_THREADS, 4) k_sample_open(int32_t* __rest
             if (top == m) at = min(at, b);
             double v = 0.0;
             if (!greedy && m == INFINITY) v = top == m ? block_mass[b] : 0.0;
-            else if (!greedy) v = block_mass[b] * weight_of(top, m, fmaxf(m - reach, -3.4028235e38f), rate, power);
+            else if (!greedy) v = block_mass[b] * weight_of(top, m, fmaxf(__fsub_ru(m, reach), -3.4028235e38f), rate, power);
             block_mass[b] = v;
             mine += v;
         }

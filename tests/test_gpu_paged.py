@@ -453,6 +453,56 @@ def test_sample_odd_logits(lib):
     assert sample(lib, x, 0.1)[[0, 3]].tolist() == [-1, -1]
 
 
+def test_sample_extreme_temperatures(lib):
+    """Temperatures at which every other logit weighs nothing, or all weigh the same; logits far from zero."""
+    rng = np.random.default_rng(11)
+    x = (rng.standard_normal((6, 9000)) * 3).astype(np.float32)
+    x[2] += 3e4
+    x[3] *= 1e30
+    x[4] = np.where(rng.random(9000) < 0.5, np.float32(1.0), np.nextafter(np.float32(1.0), np.float32(2.0)))
+    x[5, :40] = -np.inf
+    u = np.array([0.2, 0.4, 0.6, 0.8, 0.3, 0.999], np.float32)
+    for t in (1e-30, 1e-12, 1e-7, 1e-3, 50.0, 1e6, 1e30, np.inf):
+        for kw in (dict(), dict(top_k=30), dict(top_k=2000), dict(top_p=0.7), dict(min_p=0.2)):
+            got = sample(lib, x, u, temperature=t, **kw)
+            check_sample(got, x, u, temperature=t, **kw)
+
+
+def test_sample_logits_far_from_zero(lib):
+    """Neighbouring FP32 values lie further apart than the weights reach, or the range passes FP32's largest number."""
+    rng = np.random.default_rng(12)
+    v = 5003
+    x = np.zeros((6, v), np.float32)
+    steps = rng.integers(0, 6, (6, v))
+    for i, top in enumerate((1e10, 1e12, 3e38, -1e12)):
+        x[i] = top
+        for s in range(1, 6):
+            lower = np.nextafter(x[i], np.float32(-np.inf))
+            x[i] = np.where(steps[i] >= s, lower, x[i])
+    x[4] = rng.choice(np.array([3.4e38, 1e38, -3.4e38, 0], np.float32), v)
+    x[5] = -1e30
+    x[5, [17, 4000]] = np.float32(-1e12)
+    u = np.array([0.2, 0.4, 0.6, 0.8, 0.3, 0.7], np.float32)
+    for t in (1e-3, 0.7, 1.0, 2.0, 50.0, 100.0, 1000.0, 1e5, 1e37):
+        for kw in (dict(), dict(top_k=3), dict(top_k=200), dict(top_k=2000), dict(top_p=0.7), dict(min_p=0.2), dict(min_p=1e-6)):
+            check_sample(sample(lib, x, u, temperature=t, **kw), x, u, temperature=t, **kw)
+
+
+def test_sample_last_kept(lib):
+    """u = 1 and NaN take the last kept index that weighs anything, also where its weight is far below the others'."""
+    x = np.full((4, 700), -np.inf, np.float32)
+    x[:, 5] = 0.0
+    x[0, 600] = -600.0           # 2^-866
+    x[1, 600] = -800.0           # nothing
+    x[2, [300, 650]] = -60.0
+    x[3] = np.linspace(0, -650, 700)
+    for u in (1.0, 7.0, np.nan):
+        for kw in (dict(), dict(top_k=4), dict(top_k=600), dict(min_p=0.0)):
+            got = sample(lib, x, np.full(4, u, np.float32), **kw)
+            want = [600, 5, 650, min(kw.get("top_k", 700), 700) - 1]
+            assert got.tolist() == want, (u, kw)
+
+
 def test_sample_follows_the_distribution(lib):
     """Evenly spaced u hit each token in proportion to its mass, to one hit either way."""
     x = np.random.default_rng(6).standard_normal(50).astype(np.float32)
