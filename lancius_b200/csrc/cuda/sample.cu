@@ -55,8 +55,7 @@ struct Row {
     const float* x;     // this CTA's part, in shared memory, cleaned
     int padded, first;  // its length and the index of its first token
     float max, min;     // of the row, min over the finite ones
-    double top, rate;   // max, log2(e) / t
-    float nothing;      // weights are 0 below this logit
+    double top, rate;   // max, 16 log2(e) / t
     const double* power;   // 2^(j/16), in shared memory
     bool fresh;         // the histogram is cleared
     float tau;          // kept: logit > tau, or logit == tau and index <= last
@@ -79,29 +78,23 @@ __device__ __forceinline__ void for_kept(const Row& r, Use use) {
         if (kept(r, v.w, 4 * j + 3)) use(v.w, 4 * j + 3);
     }
 }
-// 2^z, z = n / 16 + f, |f| <= 1/32: a table of 2^(j/16) times the Taylor series of 2^f to f^6
-// (table-driven exponential, Tang 1989); the series' remainder is 5e-16. 13 FP64 instructions, where the library's
-// exp and a division took 124 of all kinds. For z > -1022.
-__device__ __forceinline__ double power_of_two(double z, const double* power) {
+// exp((x - top) / t), rate = 16 log2(e) / t, for weights above 2^-1022. 2^(z / 16) with z = n + f, |f| <= 1/2, is a table of
+// 2^(j/16) times a polynomial (table-driven exponential, Tang 1989): 1 + f q(f), q interpolating (2^(f/16) - 1) / f at the 5
+// Chebyshev nodes of [-1/2, 1/2]; relative error 9e-15. 10 FP64 instructions and a conversion.
+__device__ __forceinline__ double weight_of(float x, double top, double rate, const double* power) {
     constexpr double MAGIC = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the rounded integer
-    const double k = fma(z, 16.0, MAGIC);
+    const double d = (double)x - top, k = fma(d, rate, MAGIC);
     const int n = __double2loint(k);
-    const double f = fma(k - MAGIC, -0.0625, z);
-    double p = 1.5403530393381609954e-4;           // ln2^i / i!
-    p = fma(p, f, 1.3333558146428443423e-3);
-    p = fma(p, f, 9.6181291076284771620e-3);
-    p = fma(p, f, 5.5504108664821579953e-2);
-    p = fma(p, f, 2.4022650695910071233e-1);
-    p = fma(p, f, 6.9314718055994530942e-1);
+    const double f = fma(d, rate, MAGIC - k);
+    double p = 1.2716049516906705e-9;
+    p = fma(p, f, 1.4676387238435006e-7);
+    p = fma(p, f, 1.3550807778387664e-5);
+    p = fma(p, f, 9.3838479262966460e-4);
+    p = fma(p, f, 4.3321698784996580e-2);
     p = fma(p, f, 1.0) * power[n & 15];
-    return __hiloint2double(__double2hiint(p) + ((n >> 4) << 20), __double2loint(p));
+    return __hiloint2double(__double2hiint(p) + ((n & ~15) << 16), __double2loint(p));
 }
-// exp((x - top) / t) without branches; 0 below `nothing`, 2^-1000.
-__device__ __forceinline__ double weight_of(float x, double top, float nothing, double rate, const double* power) {
-    const double w = power_of_two(((double)fmaxf(x, nothing) - top) * rate, power);
-    return x >= nothing ? w : 0.0;
-}
-__device__ __forceinline__ double weight(const Row& r, float x) { return weight_of(x, r.top, r.nothing, r.rate, r.power); }
+__device__ __forceinline__ double weight(const Row& r, float x) { return weight_of(x, r.top, r.rate, r.power); }   // of a kept one
 __device__ __forceinline__ u64 fixed_weight(const Row& r, float x) {   // times 2^44, rounded
     return (u64)__double_as_longlong(fma(weight(r, x), FIXED, 4503599627370496.0)) & 0xfffffffffffffull;
 }
@@ -293,7 +286,7 @@ __device__ void finish_small(cg::cluster_group& cl, Shared& sh, const Row& r, in
         for (int j = 0; j < n; j++)
             if ((uint32_t)sh.list[j] >= (uint32_t)me) upto += sh.list_mass[j];   // indices up to this one
         if (w && (double)upto > target) atomicMin(&sh.at, index);
-        if (of_key((uint32_t)(me >> 32)) >= r.nothing) atomicMax(&sh.last, index);
+        atomicMax(&sh.last, index);
     }
     __syncthreads();
     if (tid == 0) *token = sh.at < 0x7fffffff ? sh.at : sh.last;
@@ -336,7 +329,7 @@ __device__ void finish_ties(cg::cluster_group& cl, Shared& sh, Row& r, float val
 struct ValueBins {
     float max, per;
     __device__ bool make(const Row& r) {
-        const float range = fminf(r.max - r.min, 144.f / (float)r.rate);
+        const float range = fminf(r.max - r.min, 144.f * 16 / (float)r.rate);
         max = r.max;
         per = (BINS - 1) / range;
         return range > 0.f && range < INFINITY && per < 1e30f;
@@ -414,16 +407,29 @@ __device__ __forceinline__ int or_last(int at, bool any) {
     return at < 32 ? at : 31 - __clz(some);
 }
 // One warp draws within its CTA: mine, the inclusive sums by lane of per neighbouring blocks each; block_mass, the blocks'
-// sums; lane_weights(block, w), the weights of the lane's 4 logits of a block. Returns the index in the CTA's part.
-template <typename Weights>
+// sums; lane_weights(i, w), the weights of the 4 logits of the lane in the 128 at 128 i, SUBS of which make a block.
+// Returns the index in the CTA's part.
+template <int SUBS, typename Weights>
 __device__ __forceinline__ int draw_in_part(double mine, bool mine_any, int per, int blocks, const double* block_mass, double ahead,
                                             double target, Weights lane_weights) {
     const int lane = threadIdx.x & 31;
     int at = or_last(first_over(mine, mine_any, ahead, target), mine_any);
     const int b0 = at * per, n = min(per, blocks - b0);   // per <= 8 blocks
     const double of_block = lane < n ? block_mass[b0 + lane] : 0.0;
-    const int block = b0 + or_last(first_over(scan(of_block), of_block > 0.0, ahead, target), of_block > 0.0);
+    int block = (b0 + or_last(first_over(scan(of_block), of_block > 0.0, ahead, target), of_block > 0.0)) * SUBS;
     double w[4];
+    if (SUBS > 1) {
+        double of_sub = 0.0;
+#pragma unroll
+        for (int s = 0; s < SUBS; s++) {
+            lane_weights(block + s, w);
+            double v = (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (lane == s) of_sub = v;
+        }
+        block += or_last(first_over(scan(of_sub), of_sub > 0.0, ahead, target), of_sub > 0.0);
+    }
     lane_weights(block, w);
     const double four = (w[0] + w[1]) + (w[2] + w[3]);
     at = or_last(first_over(scan(four), four > 0.0, ahead, target), four > 0.0);
@@ -454,7 +460,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
     const float t = temperature ? temperature[row] : 1.f, mp = min_p ? min_p[row] : 0.f, p = top_p ? top_p[row] : 1.f;
     const int k = top_k ? top_k[row] : 0;
     const bool greedy = !(t > 0.f), cuts = !greedy && ((k > 0 && k < vocab) || p < 1.f);
-    const double rate = 1.4426950408889634074 / (double)t;
+    const double rate = 16 * 1.4426950408889634074 / (double)t;
     float m = -INFINITY, lowest = INFINITY;   // lowest of the finite ones, where a cut will want it
     auto take = [&](float x) {
         x = clean(x);
@@ -513,14 +519,14 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
     r.fresh = true;
     r.rate = rate;
     r.power = sh.power;
-    // 2^-1000; rounded up, so that far from zero the logits next to the largest stay within the exponent's range
-    r.nothing = fmaxf(__double2float_ru(r.top - (1000.0 * 0.69314718055994530942) * (double)t), -3.4028235e38f);
-    r.tau = -3.4028235e38f;   // everything above -infinity
+    // What weighs less than 2^-1000 is not kept. Rounded up, so that far from zero no logit next to the largest leaves the
+    // exponent's range.
+    r.tau = fmaxf(__double2float_ru(r.top - (1000.0 * 0.69314718055994530942) * (double)t), -3.4028235e38f);
     r.last = ALL;
     if (mp > 0.f && t < INFINITY) {
         r.tau = fmaxf(r.tau, fminf(m, __double2float_ru((double)m + (double)t * log((double)fminf(mp, 1.f))) + 0.f));
-        r.min = fmaxf(r.min, r.tau);
     }
+    r.min = fmaxf(r.min, r.tau);
     if (k > 0 && k < vocab && cut<false>(cl, sh, r, k, p, u[row], token + row)) return;
     if (p < 1.f) cut<true>(cl, sh, r, 0, fmaxf(p, 1e-30f), 0.0, nullptr);   // rank 0 always stays
 
@@ -531,10 +537,10 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
         const bool k0 = kept(r, v.x, i), k1 = kept(r, v.y, i + 1), k2 = kept(r, v.z, i + 2), k3 = kept(r, v.w, i + 3);
         w[0] = w[1] = w[2] = w[3] = 0.0;
         if (!__any_sync(0xffffffffu, k0 || k1 || k2 || k3)) return;
-        w[0] = weight(r, k0 ? v.x : -INFINITY);
-        w[1] = weight(r, k1 ? v.y : -INFINITY);
-        w[2] = weight(r, k2 ? v.z : -INFINITY);
-        w[3] = weight(r, k3 ? v.w : -INFINITY);
+        w[0] = k0 ? weight(r, fmaxf(v.x, r.tau)) : 0.0;   // without branches
+        w[1] = k1 ? weight(r, fmaxf(v.y, r.tau)) : 0.0;
+        w[2] = k2 ? weight(r, fmaxf(v.z, r.tau)) : 0.0;
+        w[3] = k3 ? weight(r, fmaxf(v.w, r.tau)) : 0.0;
     };
     const int blocks = r.padded / BLOCK;
     for (int b = warp; b < blocks; b += WARPS) {
@@ -563,11 +569,9 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
     const double total = __shfl_sync(0xffffffffu, of_cta, 31), target = (double)u[row] * total;
     double ahead = 0.0;
     const int owner = first_over(of_cta, cta_any, ahead, target);
-    if (owner >= ranks) {   // u >= 1, or the sums' last bits: the last kept token that weighs anything
+    if (owner >= ranks) {   // u >= 1, or the sums' last bits: the last kept token
         int last = -1;
-        for_kept(r, [&](float x, int i) {
-            if (weight(r, x) > 0.0) last = max(last, r.first + i);
-        });
+        for_kept(r, [&](float, int i) { last = max(last, r.first + i); });
         last = __reduce_max_sync(0xffffffffu, last);
         __syncthreads();
         if (tid == 0) sh.last = -1;
@@ -578,7 +582,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
         return;
     }
     if (owner == rank && warp == 0) {
-        const int at = draw_in_part(mine, mine_any, per, blocks, sh.block_mass, ahead, target, lane_weights);
+        const int at = draw_in_part<1>(mine, mine_any, per, blocks, sh.block_mass, ahead, target, lane_weights);
         if (lane == 0) token[row] = r.first + at;
     }
     cl.sync();   // nobody leaves while its shared memory is read
@@ -587,21 +591,21 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
 // Without filters: one pass. Each warp takes blocks of 128 logits, whose weights are summed relative to the block's own
 // maximum; the sums are brought to the row's maximum when that is known, and the drawn block's logits are read again.
 // Nothing of a row stays in shared memory but a maximum and a sum per block, so twice as many CTAs run as above.
-constexpr int OPEN_THREADS = 256, OPEN_WARPS = OPEN_THREADS / 32;
+constexpr int OPEN_THREADS = 256, OPEN_WARPS = OPEN_THREADS / 32, OPEN_SUBS = 2, OPEN_BLOCK = OPEN_SUBS * BLOCK, OPEN_MOST = 32768;
 
 __global__ void __launch_bounds__(OPEN_THREADS, 4) k_sample_open(int32_t* __restrict__ token, const float* __restrict__ logits,
                                                                  size_t ld, int vocab, int part, int vec, const float* temperature,
                                                                  const float* u) {
-    __shared__ double block_mass[MAX_BLOCKS], power[16], mass_here;
-    __shared__ float block_max[MAX_BLOCKS], warp_max[OPEN_WARPS], max_here;
+    __shared__ double block_mass[OPEN_MOST / OPEN_BLOCK], power[16], mass_here;
+    __shared__ float block_max[OPEN_MOST / OPEN_BLOCK], warp_max[OPEN_WARPS], max_here;
     __shared__ int first_here;
     cg::cluster_group cl = cg::this_cluster();
     const int ranks = cl.num_blocks(), rank = cl.block_rank(), row = blockIdx.x / ranks, first = rank * part;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int n = max(0, min(part, vocab - first)), blocks = (n + BLOCK - 1) / BLOCK;
+    const int n = max(0, min(part, vocab - first)), blocks = (n + OPEN_BLOCK - 1) / OPEN_BLOCK;
     const float* src = logits + (size_t)row * ld + first;
     const float t = temperature ? temperature[row] : 1.f;
-    const double rate = 1.4426950408889634074 / (double)t;
+    const double rate = 16 * 1.4426950408889634074 / (double)t;
     const bool greedy = !(t > 0.f);
     if (tid < 16) power[tid] = exp2((double)tid / 16);
     if (tid == 0) first_here = ALL;
@@ -610,54 +614,59 @@ __global__ void __launch_bounds__(OPEN_THREADS, 4) k_sample_open(int32_t* __rest
         const int i = block * BLOCK + 4 * lane;
         if (vec && i + 3 < n) {
             const float4 v = *reinterpret_cast<const float4*>(src + i);
-            x[0] = clean(v.x); x[1] = clean(v.y); x[2] = clean(v.z); x[3] = clean(v.w);
+            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
         } else {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int k = vec || in_order ? i + j : block * BLOCK + 32 * j + lane;
-                x[j] = k < n ? clean(src[k]) : -INFINITY;
+                x[j] = k < n ? src[k] : -INFINITY;
             }
         }
     };
     const float reach = 693.f * t;   // 2^-1000, rounded up where it is subtracted
-    auto lane_weights = [&](const float (&x)[4], float top, double (&w)[4]) {   // relative to top
-        if (top == INFINITY) {       // the infinite ones share the mass
+    constexpr float LOWEST = -3.4028235e38f;
+    auto nothing_below = [&](float top) { return fmaxf(__fsub_ru(top, reach), LOWEST); };
+    // Weights relative to top, the largest or infinite: then the infinite ones share the mass. What lies below `nothing`
+    // weighs as much as that, or with to_zero 0.
+    auto lane_weights = [&](const float (&x)[4], float top, float nothing, bool to_zero, double (&w)[4]) {
+        if (top == INFINITY) {
 #pragma unroll
             for (int j = 0; j < 4; j++) w[j] = x[j] == INFINITY ? 1.0 : 0.0;
         } else {
-            const float nothing = fmaxf(__fsub_ru(top, reach), -3.4028235e38f);
 #pragma unroll
-            for (int j = 0; j < 4; j++) w[j] = weight_of(x[j], top, nothing, rate, power);
+            for (int j = 0; j < 4; j++) {
+                w[j] = weight_of(fmaxf(x[j], nothing), top, rate, power);
+                if (to_zero && !(x[j] >= nothing)) w[j] = 0.0;
+            }
         }
     };
-    constexpr int AHEAD = 2;   // blocks of a warp in flight
-    float x[AHEAD][4], m = -INFINITY;
+    float m = -INFINITY;
+    for (int b = warp; b < blocks; b += OPEN_WARPS) {
+        float x[OPEN_SUBS][4], top = -INFINITY;
 #pragma unroll
-    for (int a = 0; a < AHEAD; a++)
-        if (warp + a * OPEN_WARPS < blocks) fetch(warp + a * OPEN_WARPS, x[a], false);
-    for (int b0 = warp; b0 < blocks; b0 += AHEAD * OPEN_WARPS) {
+        for (int s = 0; s < OPEN_SUBS; s++) fetch(b * OPEN_SUBS + s, x[s], false);
 #pragma unroll
-        for (int a = 0; a < AHEAD; a++) {
-            const int b = b0 + a * OPEN_WARPS;
-            if (b >= blocks) break;
-            float y[4];
+        for (int s = 0; s < OPEN_SUBS; s++) top = fmaxf(top, fmaxf(fmaxf(x[s][0], x[s][1]), fmaxf(x[s][2], x[s][3])));
 #pragma unroll
-            for (int j = 0; j < 4; j++) y[j] = x[a][j];
-            if (b + AHEAD * OPEN_WARPS < blocks) fetch(b + AHEAD * OPEN_WARPS, x[a], false);
-            float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        double v = 0.0;
+        if (!greedy && top > -INFINITY) {
+            const float nothing = nothing_below(top);
+            auto add = [&](bool to_zero) {
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            double v = 0.0;
-            if (!greedy && top > -INFINITY) {
-                double w[4];
-                lane_weights(y, top, w);
-                v = (w[0] + w[1]) + (w[2] + w[3]);
+                for (int s = 0; s < OPEN_SUBS; s++) {
+                    double w[4];
+                    lane_weights(x[s], top, nothing, to_zero, w);
+                    v += (w[0] + w[1]) + (w[2] + w[3]);
+                }
+            };
+            if (reach < INFINITY && top - nothing >= 0.9f * reach) add(false);   // 2^-900 is lost in a sum with the largest's 1
+            else add(true);   // hot, or so far from zero that `nothing` was rounded far up
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            }
-            if (lane == 0) { block_max[b] = top; block_mass[b] = v; }
-            m = fmaxf(m, top);
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         }
+        if (lane == 0) { block_max[b] = top; block_mass[b] = v; }
+        m = fmaxf(m, top);
     }
     if (lane == 0) warp_max[warp] = m;
     __syncthreads();
@@ -675,6 +684,7 @@ __global__ void __launch_bounds__(OPEN_THREADS, 4) k_sample_open(int32_t* __rest
     const int per = (blocks + 31) / 32;
     if (warp == 0) {
         int at = ALL;   // the first block that holds the row's maximum
+        const float nothing = nothing_below(m);
         for (int k = 0; k < per; k++) {
             const int b = lane * per + k;
             if (b >= blocks) break;
@@ -682,7 +692,7 @@ __global__ void __launch_bounds__(OPEN_THREADS, 4) k_sample_open(int32_t* __rest
             if (top == m) at = min(at, b);
             double v = 0.0;
             if (!greedy && m == INFINITY) v = top == m ? block_mass[b] : 0.0;
-            else if (!greedy) v = block_mass[b] * weight_of(top, m, fmaxf(__fsub_ru(m, reach), -3.4028235e38f), rate, power);
+            else if (!greedy && top >= nothing) v = block_mass[b] * weight_of(top, m, rate, power);
             block_mass[b] = v;
             mine += v;
         }
@@ -692,13 +702,15 @@ __global__ void __launch_bounds__(OPEN_THREADS, 4) k_sample_open(int32_t* __rest
         if (greedy && m > -INFINITY) {
             at = __reduce_min_sync(0xffffffffu, at);
             if (at < ALL) {
-                float y[4];
-                fetch(at, y, true);
-                const int mark = y[0] == m ? 0 : y[1] == m ? 1 : y[2] == m ? 2 : y[3] == m ? 3 : ALL;
-                const unsigned hit = __ballot_sync(0xffffffffu, mark < ALL);
-                const int l = __ffs(hit) - 1;
-                const int j = __shfl_sync(0xffffffffu, mark, l);
-                if (lane == 0) first_here = first + at * BLOCK + 4 * l + j;
+                int where = ALL;
+                for (int s = 0; s < OPEN_SUBS; s++) {
+                    float y[4];
+                    fetch(at * OPEN_SUBS + s, y, true);
+                    const int j = y[0] == m ? 0 : y[1] == m ? 1 : y[2] == m ? 2 : y[3] == m ? 3 : ALL;
+                    if (j < ALL) where = min(where, BLOCK * s + 4 * lane + j);
+                }
+                where = __reduce_min_sync(0xffffffffu, where);
+                if (lane == 0) first_here = first + at * OPEN_BLOCK + where;
             }
         }
     }
@@ -716,10 +728,10 @@ __global__ void __launch_bounds__(OPEN_THREADS, 4) k_sample_open(int32_t* __rest
             // u >= 1 draws from the last that has any, and there the last
             const int owner = or_last(first_over(of_cta, cta_any, ahead, target), cta_any);
             if (owner == rank) {
-                const int at = draw_in_part(mine, mine_any, per, blocks, block_mass, ahead, target, [&](int block, double (&w)[4]) {
+                const int at = draw_in_part<OPEN_SUBS>(mine, mine_any, per, blocks, block_mass, ahead, target, [&](int block, double (&w)[4]) {
                     float y[4];
                     fetch(block, y, true);
-                    lane_weights(y, m, w);
+                    lane_weights(y, m, nothing_below(m), true, w);
                 });
                 if (lane == 0) token[row] = first + at;
             }
