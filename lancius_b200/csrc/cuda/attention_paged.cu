@@ -30,6 +30,7 @@
 // zeros by cp.async, so stale bytes never reach an MMA.
 #include "kv_paged.cuh"
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
@@ -41,13 +42,13 @@ constexpr float RAISE = 8.f;      // the running maximum moves only when exceede
 
 __device__ int g_attn_paged_fault = 0;
 
-template <int D, int ROWS>   // ROWS of q per CTA: 4, 8 or 16
+template <int D, int ROWS>   // ROWS of q per CTA: 4 or a multiple of 8
 struct Shape {
     static constexpr int ROW = D / 2, SROW = D / 16;            // code and scale bytes of a cached row
-    static constexpr int STAGES = D == 256 ? 2 : D == 128 ? (ROWS == 16 ? 3 : 2) : 4;
+    static constexpr int STAGES = D == 256 ? 2 : D == 128 ? (ROWS >= 16 ? 3 : 2) : 4;
     static constexpr int CODES = TILE * ROW, SCALES = TILE * SROW;
     static constexpr int STAGE = 2 * (CODES + SCALES);
-    static constexpr int NT = ROWS == 16 ? 2 : 1;               // 8-column operands
+    static constexpr int NT = (ROWS + 7) / 8;                   // 8-column operands
     static constexpr bool PACK = ROWS == 4;                     // hi and lo halves share one
     static constexpr int STEPS = D / 16;
     static constexpr int Q_BYTES = STEPS * (PACK ? 256 : 512) * NT;
@@ -55,7 +56,8 @@ struct Shape {
     static constexpr int O_LD = D + 4;
     static constexpr int MERGE = WARPS * ROWS * O_LD * 4;       // reuses the ring
     static constexpr int SMEM = Q_BYTES + (RING > MERGE ? RING : MERGE);
-    static constexpr int RESIDENT = D == 256 ? 2 : D == 128 ? (ROWS == 16 ? 3 : 4) : ROWS == 16 ? 4 : 5;   // CTAs per SM
+    static constexpr int RESIDENT = D == 256 ? 2 : D == 128 ? (ROWS <= 8 ? 4 : ROWS == 16 ? 3 : 2)
+                                             : ROWS <= 8 ? 5 : ROWS == 16 ? 4 : 3;   // CTAs per SM
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -176,6 +178,17 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     least = limit_of(0);                                          // positions rise with the row
     const int begin = split_id * sp.chunk, end = min(begin + sp.chunk, limit_of(cols - 1));
 
+    // q: a warp's columns are on their way together, while the first tiles are asked for
+    constexpr int QN = D / 32, QC = COLS / WARPS;
+    float qx[QC][QN];
+#pragma unroll
+    for (int k = 0; k < QC; k++) {
+        const int c = warp + k * WARPS, ci = block * COLS + c;
+        const float* from = q + (size_t)(first + ci / group) * q_ld + (size_t)(head * group + ci % group) * D + lane;
+#pragma unroll
+        for (int i = 0; i < QN; i++) qx[k][i] = c < cols ? from[32 * i] : 0.f;
+    }
+
     // loads: tile i of this warp holds keys begin + 32 (warp + 4 i) ...
     const int tiles_all = end > begin ? (end - begin + TILE - 1) / TILE : 0;
     const int tiles = tiles_all > warp ? (tiles_all - warp + WARPS - 1) / WARPS : 0;
@@ -234,15 +247,13 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 
     // q as B fragments in shared memory: [8 rows][step][lane][hi 0, hi 1, lo 0, lo 1]; packed: [step][lane][2], columns 0-3
     // hi, 4-7 lo
-    for (int c = warp; c < COLS; c += WARPS) {
-        constexpr int N = D / 32;
-        const int ci = block * COLS + c;
-        float x[N], amax = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            x[i] = c < cols ? q[(size_t)(first + ci / group) * q_ld + (size_t)(head * group + ci % group) * D + lane + 32 * i] : 0.f;
-            amax = fmaxf(amax, fabsf(x[i]));
-        }
+    for (int k = 0; k < QC; k++) {
+        const int c = warp + k * WARPS;
+        const float(&x)[QN] = qx[k];
+        float amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < QN; i++) amax = fmaxf(amax, fabsf(x[i]));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         int e = (int)(__float_as_uint(amax) >> 23) - 127;          // 2^e <= amax < 2^(e + 1)
@@ -252,7 +263,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
         if (lane == 0) col_scale[c] = scale_log2 * 16.f * p.k_unit * up;   // K comes as value / 16
         __half* frag = reinterpret_cast<__half*>(smem);
 #pragma unroll
-        for (int i = 0; i < N; i++) {
+        for (int i = 0; i < QN; i++) {
             const int ch = lane + 32 * i, owner = ch / (D / 4), in = ch % (D / 4), step = in / 8 * 2 + ((in & 3) >> 1);
             const float y = x[i] * down;
             const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
@@ -635,10 +646,31 @@ __global__ void __launch_bounds__(THREADS) k_attn_paged_join(float* __restrict__
 
 lancius_error bad(lancius_error e) { lancius_set_error(e); return e; }
 
-size_t row_blocks(int rows) { return rows > 8 ? ((size_t)rows + 15) / 16 : 1; }
+// Rows of q per CTA. Up to 4 fit one operand with both halves of q (half the MMAs); more rows share the cost of turning
+// the codes into operands, as far as the accumulators allow. Rows over that are spread evenly.
+int block_rows(int D, int rows) {
+    if (rows <= 4) return 4;
+    const int most = D == 256 ? 16 : 24, n = (rows + most - 1) / most;
+    return ((rows + n - 1) / n + 7) / 8 * 8;
+}
+size_t row_blocks(int D, int rows) { const int n = block_rows(D, rows); return ((size_t)rows + n - 1) / n; }
 
-template <int D>
-int resident(int rows) { return rows <= 8 ? Shape<D, 8>::RESIDENT : Shape<D, 16>::RESIDENT; }
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+// f(Int<D>, Int<rows of q per CTA>)
+template <typename F>
+auto with_shape(int D, int rows, F f) {
+    const int n = block_rows(D, rows);
+    auto of = [&](auto d) {
+        constexpr int C = decltype(d)::value;
+        if (n == 4) return f(d, Int<4>());
+        if (n == 8) return f(d, Int<8>());
+        if constexpr (C <= 128) if (n == 24) return f(d, Int<24>());
+        return f(d, Int<16>());
+    };
+    return D == 64 ? of(Int<64>()) : D == 128 ? of(Int<128>()) : of(Int<256>());
+}
 
 // Keys per CTA. Few keys: every CTA that fits on the GPU gets one chunk (131072 keys of one sequence, 8 heads: 47.5 us in
 // one round of CTAs, 54.9 in two, 66.7 in three). Many keys: rounds of at most 1536, as short ones cost more starts
@@ -647,8 +679,8 @@ int resident(int rows) { return rows <= 8 ? Shape<D, 8>::RESIDENT : Shape<D, 16>
 // warp.
 Split plan(const KvPagesDev& p, const KvBatchDev& b, int D, int group) {
     const int rows = group * b.max_new;
-    const size_t slots = (size_t)LCU_SMS * (D == 256 ? resident<256>(rows) : D == 128 ? resident<128>(rows) : resident<64>(rows));
-    const size_t ctas = (size_t)b.n_seqs * p.heads * row_blocks(rows), len = b.max_len > 0 ? b.max_len : 1;
+    const size_t slots = LCU_SMS * with_shape(D, rows, [](auto d, auto n) { return (size_t)Shape<d, n>::RESIDENT; });
+    const size_t ctas = (size_t)b.n_seqs * p.heads * row_blocks(D, rows), len = b.max_len > 0 ? b.max_len : 1;
     const size_t keys = len * ctas / 4 * (b.n_seqs > 1 ? 3 : 4);
     size_t chunk = (keys + slots - 1) / slots;
     if (chunk > MAX_CHUNK) chunk /= (chunk + 1535) / 1536;
@@ -667,7 +699,7 @@ lancius_error check_call(const lcu_kv_pages* pages, const lcu_kv_batch* batch, s
         n_q_heads / pages->n_heads * b->max_new > (size_t)INT32_MAX / 2)
         return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
     const Split sp = plan(*p, *b, (int)pages->head_dim, (int)(n_q_heads / pages->n_heads));
-    if ((size_t)sp.splits * row_blocks((int)(n_q_heads / pages->n_heads) * b->max_new) > (size_t)INT32_MAX ||
+    if ((size_t)sp.splits * row_blocks((int)pages->head_dim, (int)(n_q_heads / pages->n_heads) * b->max_new) > (size_t)INT32_MAX ||
         part_rows(*b, n_q_heads, sp) > (size_t)1 << 40)
         return bad(LANCIUS_ERROR_SHAPE_MISMATCH);
     return LANCIUS_ERROR_OK;
@@ -680,7 +712,7 @@ lancius_error launch(float* out, const float* q, size_t q_ld, int hq, const KvPa
     static std::atomic<unsigned long long> allowed{0};   // devices on which the kernel may use its shared memory
     cudaError_t ce = lcu_allow_smem(allowed, k_attn_paged<D, ROWS>, S::SMEM);
     if (ce != cudaSuccess) return lcu_check_cuda(ce);
-    const dim3 grid((unsigned)(sp.splits * row_blocks(hq / p.heads * b.max_new)), (unsigned)p.heads, (unsigned)b.n_seqs);
+    const dim3 grid((unsigned)(sp.splits * row_blocks(D, hq / p.heads * b.max_new)), (unsigned)p.heads, (unsigned)b.n_seqs);
     k_attn_paged<D, ROWS><<<grid, THREADS, S::SMEM, st>>>(out, q, q_ld, hq, p, b, (float)(1.4426950408889634 / sqrt((double)D)), sp,
                                                           part_o, part_ml);
     lcu_note_launch();
@@ -703,16 +735,6 @@ lancius_error launch(float* out, const float* q, size_t q_ld, int hq, const KvPa
     }
     lcu_note_launch();
     return lcu_launch_status();
-}
-
-// rows of a key head: up to 4 fit one operand with both halves of q (half the MMAs), up to 8 one operand per half
-template <int D>
-lancius_error launch_rows(float* out, const float* q, size_t q_ld, int hq, const KvPagesDev& p, const KvBatchDev& b, Split sp,
-                          float* part_o, float2* part_ml, cudaStream_t st) {
-    const int rows = hq / p.heads * b.max_new;
-    if (rows <= 4) return launch<D, 4>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
-    if (rows <= 8) return launch<D, 8>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
-    return launch<D, 16>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
 }
 
 }  // namespace
@@ -755,9 +777,8 @@ lancius_error lcu_attention_paged(float* out, const float* q, size_t q_ld, size_
         part_ml = reinterpret_cast<float2*>(part_o + rows * D);
     }
     cudaStream_t st = lcu_as_stream(stream);
-    if (D == 64) return launch_rows<64>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
-    if (D == 128) return launch_rows<128>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
-    return launch_rows<256>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
+    return with_shape((int)D, hq / p.heads * b.max_new,
+                      [&](auto d, auto n) { return launch<d, n>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st); });
 }
 
 }  // extern "C"

@@ -44,7 +44,7 @@ struct Shared {
     u64 list[LIST], list_mass[LIST];   // key << 32 | ~index, so that larger means an earlier rank
     double power[16];
     u64 warp_sum[WARPS];
-    double block_mass[MAX_BLOCKS], mass_here;
+    double block_mass[MAX_BLOCKS], mass_of[MAX_CLUSTER];   // mass_of: written by every CTA of the cluster
     float max, min, tau;
     int at, found, bin, last;
     uint32_t listed;
@@ -334,7 +334,7 @@ struct ValueBins {
         per = (BINS - 1) / range;
         return range > 0.f && range < INFINITY && per < 1e30f;
     }
-    __device__ __forceinline__ int operator()(float x) const { return min(BINS - 1, __float2int_rz((max - x) * per)); }
+    __device__ __forceinline__ int operator()(float x) const { return __float_as_int(fminf((max - x) * per, BINS - 1) + 8388608.f) & 0xffff; }   // rounded by adding 2^23
 };
 
 // Moves the row's cut to the rank at which the running count (MASS = false: k) or mass (p times the mass of what is
@@ -560,10 +560,11 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
             if (lane * per + k < blocks) mine += sh.block_mass[lane * per + k];
         mine_any = mine > 0.0;
         mine = scan(mine);
-        if (lane == 31) sh.mass_here = mine;
+        const double here = __shfl_sync(0xffffffffu, mine, 31);
+        if (lane < ranks) cl.map_shared_rank(&sh, lane)->mass_of[rank] = here;
     }
     cl.sync();
-    double of_cta = lane < ranks ? cl.map_shared_rank(&sh, lane % ranks)->mass_here : 0.0;
+    double of_cta = lane < ranks ? sh.mass_of[lane] : 0.0;
     const bool cta_any = of_cta > 0.0;
     of_cta = scan(of_cta);
     const double total = __shfl_sync(0xffffffffu, of_cta, 31), target = (double)u[row] * total;
@@ -585,7 +586,6 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
         const int at = draw_in_part<1>(mine, mine_any, per, blocks, sh.block_mass, ahead, target, lane_weights);
         if (lane == 0) token[row] = r.first + at;
     }
-    cl.sync();   // nobody leaves while its shared memory is read
 }
 
 // Without filters: one pass. Each warp takes blocks of 128 logits, whose weights are summed relative to the block's own
