@@ -140,7 +140,7 @@ struct Split { int chunk, splits; };
 
 template <int D, int ROWS>
 __global__ void __launch_bounds__(THREADS, Shape<D, ROWS>::RESIDENT)
-k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, int hq, KvPagesDev p, KvBatchDev b,
+k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, bool q_wide, int hq, KvPagesDev p, KvBatchDev b,
              float scale_log2, Split sp, float* __restrict__ part_o, float2* __restrict__ part_ml) {
     using S = Shape<D, ROWS>;
     constexpr int COLS = ROWS, NT = S::NT, R = 2 * NT;
@@ -178,15 +178,25 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     least = limit_of(0);                                          // positions rise with the row
     const int begin = split_id * sp.chunk, end = min(begin + sp.chunk, limit_of(cols - 1));
 
-    // q: a warp's columns are on their way together, while the first tiles are asked for
-    constexpr int QN = D / 32, QC = COLS / WARPS;
-    float qx[QC][QN];
+    // q: a lane takes 8 channels, on their way while the first tiles are asked for
+    constexpr int LANES = D / 8, QC = (COLS * LANES + THREADS - 1) / THREADS;   // lanes of a row, rows of a lane
+    const int q_owner = lane % LANES & 3, q_octet = lane % LANES >> 2;
+    auto q_col = [&](int k) { return (warp + k * WARPS) * (32 / LANES) + lane / LANES; };
+    float qx[QC][8];
 #pragma unroll
     for (int k = 0; k < QC; k++) {
-        const int c = warp + k * WARPS, ci = block * COLS + c;
-        const float* from = q + (size_t)(first + ci / group) * q_ld + (size_t)(head * group + ci % group) * D + lane;
+        const int c = q_col(k), ci = block * COLS + c;
+        const float* from = q + (size_t)(first + ci / group) * q_ld + (size_t)(head * group + ci % group) * D + q_owner * (D / 4) + q_octet * 8;
 #pragma unroll
-        for (int i = 0; i < QN; i++) qx[k][i] = c < cols ? from[32 * i] : 0.f;
+        for (int i = 0; i < 8; i++) qx[k][i] = 0.f;
+        if (c < cols && q_wide) {
+            const float4 u = *reinterpret_cast<const float4*>(from), v = *reinterpret_cast<const float4*>(from + 4);
+            qx[k][0] = u.x; qx[k][1] = u.y; qx[k][2] = u.z; qx[k][3] = u.w;
+            qx[k][4] = v.x; qx[k][5] = v.y; qx[k][6] = v.z; qx[k][7] = v.w;
+        } else if (c < cols) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) qx[k][i] = from[i];
+        }
     }
 
     // loads: tile i of this warp holds keys begin + 32 (warp + 4 i) ...
@@ -246,35 +256,34 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     uint32_t row_ahead = ahead[S::STAGES - 1];
 
     // q as B fragments in shared memory: [8 rows][step][lane][hi 0, hi 1, lo 0, lo 1]; packed: [step][lane][2], columns 0-3
-    // hi, 4-7 lo
+    // hi, 4-7 lo. Of 8 channels 0, 4, 1, 5 are one step's and 2, 6, 3, 7 the next one's.
 #pragma unroll
     for (int k = 0; k < QC; k++) {
-        const int c = warp + k * WARPS;
-        const float(&x)[QN] = qx[k];
+        const int c = q_col(k);
+        const float(&x)[8] = qx[k];
         float amax = 0.f;
 #pragma unroll
-        for (int i = 0; i < QN; i++) amax = fmaxf(amax, fabsf(x[i]));
+        for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[i]));
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        for (int i = LANES / 2; i > 0; i >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, i));
         int e = (int)(__float_as_uint(amax) >> 23) - 127;          // 2^e <= amax < 2^(e + 1)
         if (amax == 0.f || e > 127) e = 0;
         e = min(max(e, -126), 126);
         const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
-        if (lane == 0) col_scale[c] = scale_log2 * 16.f * p.k_unit * up;   // K comes as value / 16
-        __half* frag = reinterpret_cast<__half*>(smem);
+        if (c >= COLS) continue;
+        if (lane % LANES == 0) col_scale[c] = scale_log2 * 16.f * p.k_unit * up;   // K comes as value / 16
 #pragma unroll
-        for (int i = 0; i < QN; i++) {
-            const int ch = lane + 32 * i, owner = ch / (D / 4), in = ch % (D / 4), step = in / 8 * 2 + ((in & 3) >> 1);
-            const float y = x[i] * down;
-            const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
-            const int at = ((((c >> 3) * S::STEPS + step) * 32 + (c & 7) * 4 + owner) * 4 + (in & 1)) * 2 + ((in >> 2) & 1);
+        for (int u = 0; u < 2; u++) {
+            uint4 f;
+            split(x[2 * u] * down, x[2 * u + 4] * down, f.x, f.z);
+            split(x[2 * u + 1] * down, x[2 * u + 5] * down, f.y, f.w);
+            const int step = 2 * q_octet + u;
             if (PACK) {
-                const int at2 = ((step * 32 + c * 4 + owner) * 2 + (in & 1)) * 2 + ((in >> 2) & 1);
-                frag[at2] = hi;
-                frag[at2 + 64] = lo;   // 16 lanes on
+                uint2* to = reinterpret_cast<uint2*>(smem) + step * 32 + c * 4 + q_owner;
+                to[0] = make_uint2(f.x, f.y);
+                to[16] = make_uint2(f.z, f.w);
             } else {
-                frag[at] = hi;
-                frag[at + 4] = lo;
+                reinterpret_cast<uint4*>(smem)[((c >> 3) * S::STEPS + step) * 32 + (c & 7) * 4 + q_owner] = f;
             }
         }
     }
@@ -713,7 +722,7 @@ lancius_error launch(float* out, const float* q, size_t q_ld, int hq, const KvPa
     cudaError_t ce = lcu_allow_smem(allowed, k_attn_paged<D, ROWS>, S::SMEM);
     if (ce != cudaSuccess) return lcu_check_cuda(ce);
     const dim3 grid((unsigned)(sp.splits * row_blocks(D, hq / p.heads * b.max_new)), (unsigned)p.heads, (unsigned)b.n_seqs);
-    k_attn_paged<D, ROWS><<<grid, THREADS, S::SMEM, st>>>(out, q, q_ld, hq, p, b, (float)(1.4426950408889634 / sqrt((double)D)), sp,
+    k_attn_paged<D, ROWS><<<grid, THREADS, S::SMEM, st>>>(out, q, q_ld, q_ld % 4 == 0 && (uintptr_t)q % 16 == 0, hq, p, b, (float)(1.4426950408889634 / sqrt((double)D)), sp,
                                                           part_o, part_ml);
     lcu_note_launch();
     if (sp.splits == 1) return lcu_launch_status();
