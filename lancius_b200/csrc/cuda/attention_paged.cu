@@ -595,13 +595,16 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     }
 }
 
-// out row = sum over its chunks of 2^(m - M) o / sum of 2^(m - M) l; one CTA per row, a warp per fourth chunk
-template <int D>
-__global__ void __launch_bounds__(THREADS) k_attn_paged_join(float* __restrict__ out, int hq, KvBatchDev b, float v_unit, Split sp,
-                                                             const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
-    constexpr int N = D / 32;
-    __shared__ float sm_l[WARPS];
-    __shared__ float sm_o[WARPS][D];
+// out row = sum over its chunks of 2^(m - M) o / sum of 2^(m - M) l; one CTA of JOIN warps per row, chunk c is warp
+// c % JOIN's. A warp asks for 8 chunks before it knows their weights.
+template <int D, int JOIN>
+__global__ void __launch_bounds__(32 * JOIN) k_attn_paged_join(float* __restrict__ out, int hq, KvBatchDev b, float v_unit, Split sp,
+                                                               const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
+    constexpr int N = D / 32, BATCH = 8;
+    using Piece = std::conditional_t<N == 2, float2, float4>;
+    constexpr int PIECES = N * 4 / (int)sizeof(Piece), W = sizeof(Piece) / 4;
+    __shared__ float sm_l[JOIN];
+    __shared__ __align__(16) float sm_o[JOIN][D];
     const int s = blockIdx.z, i = blockIdx.y, h = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int first, count;
     kv_new_tokens(b, s, first, count);
@@ -610,7 +613,16 @@ __global__ void __launch_bounds__(THREADS) k_attn_paged_join(float* __restrict__
     if (i >= count || parts <= 1) return;
     const size_t row = (size_t)(first + i) * hq + h;
     const float2* ml = part_ml + row * sp.splits;
-    const float* po = part_o + row * sp.splits * D + lane;
+    const float* po = part_o + row * sp.splits * D + lane * W;
+    Piece v[BATCH][PIECES];
+    auto fetch = [&](int c0) {
+#pragma unroll
+        for (int x = 0; x < BATCH; x++)
+            if (c0 + x * JOIN < parts)
+#pragma unroll
+                for (int y = 0; y < PIECES; y++) v[x][y] = *reinterpret_cast<const Piece*>(po + (size_t)(c0 + x * JOIN) * D + 32 * W * y);
+    };
+    fetch(warp);
     float M = -INFINITY;   // every warp finds the maximum by itself
     for (int c = lane; c < parts; c += 32) M = fmaxf(M, ml[c].x);
 #pragma unroll
@@ -618,37 +630,37 @@ __global__ void __launch_bounds__(THREADS) k_attn_paged_join(float* __restrict__
     float l = 0.f, o[N];
 #pragma unroll
     for (int n = 0; n < N; n++) o[n] = 0.f;
-    // warp w takes chunks w, w + 4, ...: 32 of their weights at a time, one per lane
-    for (int c0 = warp; c0 < parts; c0 += 32 * WARPS) {
-        const int c = c0 + lane * WARPS;
+    for (int c0 = warp; c0 < parts; c0 += BATCH * JOIN) {
+        if (c0 > warp) fetch(c0);
+        const int c = c0 + lane * JOIN;
         float f = 0.f;
-        if (c < parts) {
-            const float2 v = ml[c];
-            f = v.x == -INFINITY ? 1.f : ex2(v.x - M);   // a chunk without a visible key holds zeros (or NaN)
-            l += f * v.y;
+        if (lane < BATCH && c < parts) {
+            const float2 w = ml[c];
+            f = w.x == -INFINITY ? 1.f : ex2(w.x - M);   // a chunk without a visible key holds zeros (or NaN)
+            l += f * w.y;
         }
-        const int n_here = min(32, (parts - c0 + WARPS - 1) / WARPS);
-#pragma unroll 4
-        for (int x = 0; x < n_here; x++) {
-            const float fx = __shfl_sync(0xffffffffu, f, x);
 #pragma unroll
-            for (int n = 0; n < N; n++) o[n] = fmaf(fx, po[(size_t)(c0 + x * WARPS) * D + 32 * n], o[n]);
+        for (int x = 0; x < BATCH; x++) {
+            const float fx = __shfl_sync(0xffffffffu, f, x);
+            if (c0 + x * JOIN < parts)
+#pragma unroll
+                for (int n = 0; n < N; n++) o[n] = fmaf(fx, reinterpret_cast<const float*>(&v[x][n / W])[n % W], o[n]);
         }
     }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
     if (lane == 0) sm_l[warp] = l;
 #pragma unroll
-    for (int n = 0; n < N; n++) sm_o[warp][lane + 32 * n] = o[n];
+    for (int n = 0; n < N; n++) sm_o[warp][lane * W + n / W * 32 * W + n % W] = o[n];
     __syncthreads();
     float L = 0.f;
 #pragma unroll
-    for (int w = 0; w < WARPS; w++) L += sm_l[w];
+    for (int w = 0; w < JOIN; w++) L += sm_l[w];
     const float inv = L == 0.f ? 0.f : 16.f * v_unit / L;
-    for (int d = threadIdx.x; d < D; d += THREADS) {
+    for (int d = threadIdx.x; d < D; d += 32 * JOIN) {
         float acc = 0.f;
 #pragma unroll
-        for (int w = 0; w < WARPS; w++) acc += sm_o[w][d];
+        for (int w = 0; w < JOIN; w++) acc += sm_o[w][d];
         out[row * D + d] = acc * inv;
     }
 }
@@ -733,11 +745,12 @@ lancius_error launch(float* out, const float* q, size_t q_ld, int hq, const KvPa
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // starts while the chunks finish
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3((unsigned)hq, (unsigned)b.max_new, (unsigned)b.n_seqs);
-    cfg.blockDim = dim3(THREADS);
+    const bool many = sp.splits > 16;
+    cfg.blockDim = dim3(many ? 512 : 128);
     cfg.stream = st;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    ce = cudaLaunchKernelEx(&cfg, k_attn_paged_join<D>, out, hq, b, p.v_unit, sp, (const float*)part_o, (const float2*)part_ml);
+    ce = cudaLaunchKernelEx(&cfg, many ? k_attn_paged_join<D, 16> : k_attn_paged_join<D, 4>, out, hq, b, p.v_unit, sp, (const float*)part_o, (const float2*)part_ml);
     if (ce != cudaSuccess) {
         cudaGetLastError();
         return lcu_check_cuda(ce);
