@@ -436,28 +436,35 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
             for (int x = 0; x < 8; x++)
                 a[nt][x >> 2][x & 3] = a_hi[0][nt][x >> 2][x & 3] + (HALVES == 2 ? a_hi[HALVES - 1][nt][x >> 2][x & 3] : 0.f) +
                                        (PACK ? 0.f : a_lo[nt][x >> 2][x & 3]);
-        if (PACK) {   // hi + lo columns
+        if (PACK) {   // hi + lo columns: t < 2 adds up and weighs the first 16 keys, its partner t ^ 2 the others
 #pragma unroll
-            for (int x = 0; x < 8; x++) a[0][x >> 2][x & 3] += __shfl_xor_sync(0xffffffffu, a[0][x >> 2][x & 3], 2);
+            for (int x = 0; x < 4; x++) {
+                const float other = __shfl_xor_sync(0xffffffffu, t < 2 ? a[0][1][x] : a[0][0][x], 2);
+                a[0][0][x] = (t < 2 ? a[0][0][x] : a[0][1][x]) + other;
+            }
         }
 
-        // ---- weights. Value x of a row: key key0 + 16 (x >> 1) + 8 (x & 1) + g
-        float sv[R][4], top[R];
+        // ---- weights. Value x of a row: key key1 + 16 (x >> 1) + 8 (x & 1)
+        constexpr int X = PACK ? 2 : 4;
+        const int key1 = key0 + g + (PACK && t >= 2 ? 16 : 0);
+        float sv[R][X], top[R];
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int x = 0; x < 4; x++) sv[r][x] = a[r >> 1][x >> 1][2 * (x & 1) + (r & 1)];   // times cs[r]: log2 units
+            for (int x = 0; x < X; x++) sv[r][x] = a[r >> 1][x >> 1][2 * (x & 1) + (r & 1)];   // times cs[r]: log2 units
         if (key0 + TILE > least) {
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int x = 0; x < 4; x++)
-                    if (key0 + 8 * x + g >= limit[r]) sv[r][x] = -INFINITY;
+                for (int x = 0; x < X; x++)
+                    if (key1 + 8 * x >= limit[r]) sv[r][x] = -INFINITY;
         }
         bool raise = false;
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            top[r] = fmaxf(fmaxf(sv[r][0], sv[r][1]), fmaxf(sv[r][2], sv[r][3])) * cs[r];
+            top[r] = fmaxf(sv[r][0], sv[r][1]);
+            if (X == 4) top[r] = fmaxf(top[r], fmaxf(sv[r][X - 2], sv[r][X - 1]));
+            top[r] *= cs[r];
             raise = raise || top[r] > m[r] + RAISE;
         }
         if (__any_sync(0xffffffffu, raise)) {   // some key exceeds its row's maximum by enough
@@ -465,7 +472,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 #pragma unroll
             for (int r = 0; r < R; r++) {
 #pragma unroll
-                for (int x = 4; x < 32; x <<= 1) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], x));
+                for (int x = PACK ? 2 : 4; x < 32; x = x == 2 ? 4 : 2 * x) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], x));
                 const float mx = fmaxf(m[r], top[r]);
                 f[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - mx);   // nothing was summed before the first key
                 m[r] = mx;
@@ -481,24 +488,41 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
         uint32_t hi[NT][4], lo[NT][4];   // P^T fragments of keys 8 x ...
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            float pw[2][4];
+            float pw[2][X];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int r = 2 * nt + u;
                 const float base = m[r] == -INFINITY ? 0.f : m[r] - P_BIAS;
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    pw[u][x] = ex2(fmaf(sv[r][x], cs[r], -base));
-                    if (poison && (poison >> (8 * x + g) & 1) && key0 + 8 * x + g < limit[r]) pw[u][x] = NAN;
-                    l[r] += pw[u][x];
-                }
+                for (int x = 0; x < X; x++) pw[u][x] = ex2(fmaf(sv[r][x], cs[r], -base));
+            }
+            if (poison) {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int x = 0; x < X; x++)
+                        if ((poison >> (key1 - key0 + 8 * x) & 1) && key1 + 8 * x < limit[2 * nt + u]) pw[u][x] = NAN;
             }
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                split(pw[0][x], pw[1][x], hi[nt][x], lo[nt][x]);
-                if (PACK) hi[nt][x] = t < 2 ? hi[nt][x] : lo[nt][x];
-                hi[nt][x] = transpose8(hi[nt][x]);
-                if (!PACK) lo[nt][x] = transpose8(lo[nt][x]);
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int x = 0; x < X; x++) l[2 * nt + u] += pw[u][x];
+            if (PACK) {   // t < 2 gets the hi halves of all 32 keys, t >= 2 the lo halves
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    uint32_t h, k;
+                    split(pw[0][x], pw[1][x], h, k);
+                    const uint32_t other = __shfl_xor_sync(0xffffffffu, t < 2 ? k : h, 2);
+                    hi[nt][x] = transpose8(t < 2 ? h : other);
+                    hi[nt][2 + x] = transpose8(t < 2 ? other : k);
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < X; x++) {
+                    split(pw[0][x], pw[1][x], hi[nt][x], lo[nt][x]);
+                    hi[nt][x] = transpose8(hi[nt][x]);
+                    lo[nt][x] = transpose8(lo[nt][x]);
+                }
             }
         }
 
@@ -548,7 +572,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 #pragma unroll
     for (int r = 0; r < R; r++) {
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
+        for (int x = PACK ? 2 : 4; x < 32; x = x == 2 ? 4 : 2 * x) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
         const int c = row_at(r);
         if (g == 0) { sm_m[warp][c] = m[r]; sm_l[warp][c] = l[r]; }
     }
