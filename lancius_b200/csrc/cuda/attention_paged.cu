@@ -35,7 +35,9 @@
 namespace {
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS, TILE = 32;
-constexpr int MAX_CHUNK = 2048;   // keys of a CTA: 512 per warp, so that an FP32 accumulator takes 32 truncated sums
+// Keys of a CTA, at most, where all run at once and in rounds. An MMA truncates its sum, and a warp of the CTA adds a
+// fourth of them up in one accumulator.
+constexpr int MAX_CHUNK = 2048, ROUND = 1280;
 constexpr float P_BIAS = 7.f;     // p = 2^(s - m + 7): more of the small weights stay above f16's smallest step
 constexpr uint32_t NONE = 0xffffffffu;
 constexpr float RAISE = 8.f;      // the running maximum moves only when exceeded by 2^8: p <= 2^15 fits f16
@@ -717,22 +719,23 @@ auto with_shape(int D, int rows, F f) {
     return D == 64 ? of(Int<64>()) : D == 128 ? of(Int<128>()) : of(Int<256>());
 }
 
-// Keys per CTA. Few keys: every CTA that fits on the GPU gets one chunk (131072 keys of one sequence, 8 heads: 47.5 us in
-// one round of CTAs, 54.9 in two, 66.7 in three). Many keys: rounds of at most 1536, as short ones cost more starts
-// and joins and long ones an idle end (32 sequences of up to 8192 keys, 8 heads: 85.7 us with 256 keys, 70 with 1024 to
-// 1536, 74.9 with 2048). Sequences of a batch are taken as three quarters of the longest. A multiple of one tile per
-// warp.
+// Keys per CTA. Few keys: every CTA that fits on the GPU gets one chunk (131072 keys of one sequence, 8 heads of 128, when
+// first measured: 47.5 us in one round of CTAs, 54.9 in two, 66.7 in three). Many keys: rounds of at most ROUND, as short
+// ones cost more starts and joins and long ones an idle end (64 sequences of up to 8000 keys, 8 heads with 8 rows: 146.8 us
+// with 512 keys, 137.4 with 1024, 135.6 with 1280, 135.8 with 1536; 32 of up to 8192, 8 heads with one: 71.0, 69.3, 69.2,
+// 70.6). Sequences of a batch are taken as three quarters of the longest. A multiple of one tile per warp.
 Split plan(const KvPagesDev& p, const KvBatchDev& b, int D, int group) {
     const int rows = group * b.max_new;
     const size_t slots = LCU_SMS * with_shape(D, rows, [](auto d, auto n) { return (size_t)Shape<d, n>::RESIDENT; });
     const size_t ctas = (size_t)b.n_seqs * p.heads * row_blocks(D, rows), len = b.max_len > 0 ? b.max_len : 1;
     const size_t keys = len * ctas / 4 * (b.n_seqs > 1 ? 3 : 4);
     size_t chunk = (keys + slots - 1) / slots;
-    if (chunk > MAX_CHUNK) chunk /= (chunk + 1535) / 1536;
+    const size_t most = D == 256 ? ROUND : MAX_CHUNK;
+    if (chunk > most) chunk /= (chunk + ROUND - 1) / ROUND;
     constexpr size_t STEP = TILE * WARPS;
     chunk = (chunk + STEP - 1) / STEP * STEP;
     if (chunk < STEP) chunk = STEP;
-    if (chunk > MAX_CHUNK) chunk = MAX_CHUNK;
+    if (chunk > most) chunk = most;
     return Split{(int)chunk, (int)((len + chunk - 1) / chunk)};
 }
 size_t part_rows(const KvBatchDev& b, size_t hq, Split sp) { return (size_t)b.n_tokens * hq * sp.splits; }
