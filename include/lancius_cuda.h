@@ -294,9 +294,10 @@ size_t lcu_attention_paged_workspace(const lcu_kv_pages* pages, const lcu_kv_bat
  *   the mass of the ranks before it < top_p * the mass so kept (>= 1: off; rank 0 always stays),
  * and draws the first index at which the running mass of the kept ones, by rising index,
  * exceeds u * their mass (u in [0, 1); u >= 1 or NaN gives the last kept index that has any).
- * A weight below 2^-1000 of the largest counts as zero. temperature <= 0 or NaN takes the largest logit, the lowest index among equals. NaN logits count as -infinity; a row that
- * has nothing above -infinity gives -1. Masses are summed in 64 bits and do not depend on
- * the order in which the GPU runs. */
+ * A weight below 2^-1000 of the largest counts as zero. temperature <= 0 or NaN takes the
+ * largest logit, the lowest index among equals. NaN logits count as -infinity; a row that has
+ * nothing above -infinity gives -1. Masses are summed in 64 bits and do not depend on the
+ * order in which the GPU runs. */
 lancius_error lcu_sample(int32_t* token, const float* logits, size_t ld, size_t rows, size_t vocab,
                          const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                          const float* u, void* stream);

@@ -3,9 +3,18 @@
 // out[t][h] = sum_j p_j V_j, p = softmax(q . K_j / sqrt(D)), j = 0 .. position of row t, in one pass over the
 // cache with a running maximum and sum per row.
 //
-// Bound: HBM. A key/value pair of one head is D + D / 8 bytes and is read once for all rows of its key head
-// ((new token, query head) pairs, up to 8 or 16 per CTA); at the measured copy rate an SM receives about 46
-// codes a clock, so turning codes into operands is the work that has to fit beside the loads.
+// Bound: the floor is HBM. A key/value pair of one head is D + D / 8 bytes and is read once for all rows of its key
+// head ((new token, query head) pairs, up to 24 per CTA); at the measured copy rate an SM receives about 46 codes a
+// clock, so turning codes into operands is the work that has to fit beside the loads. What bounds the kernel is the
+// issue of that work: 760 instructions a warp and tile of 32 keys of 128 with up to 4 rows, 800 with 8, in which the
+// tensor pipe is busy for 21 and 38 %. Four warps a quarter of an SM issue them at nine tenths of the rate within the
+// loop, at 61 % over the kernel, as a CTA spends a quarter of its time on lengths, first loads and its merge. MMAs
+// do not overlap with the half-rate LOP3 and HFMA2 (18.3 clocks for a group with its MMA, 9.5 without).
+//   131072 keys of one sequence, 8 key heads of 128, 4 rows each: 40.7 us, 3.7 TB/s (0.57 of the measured copy rate)
+//   32 sequences of up to 8192 keys, 8 key heads of 128, one row each: 66.4 us, 3.55 TB/s (0.54)
+//   64 sequences of up to 8000 keys, 8 key heads of 128, 8 rows each: 133 us, 3.4 TB/s (0.51); the loads alone 83 us
+//   24 sequences of up to 3001 keys, 4 key heads of 64, 20 rows each: 19.5 us
+//   16 sequences of up to 5000 keys, one key head of 256, 8 rows: 12.9 us
 //
 // Products run as mma.sync m16n8k16 (f16 in, FP32 out). Measured 0.5 of them per clock and SM; two serve 256 codes
 // and 8 rows, so 64 codes a clock, above the HBM rate. tcgen05 would need the operands written to shared or tensor
@@ -13,7 +22,8 @@
 // (n - 8) * scale has 8 significant bits, so K and V fit f16 as they are; q (scaled to [1, 2) by a power of two) and p are
 // split into two f16 halves, 22 bits, one MMA each. The codes are operand A (16 keys or 16 channels), q and p operand B (8
 // rows): of the two assignments the one whose accumulator for O is half as large, which decides how many warps
-// fit (measured with q and p as A, halves stacked in its 16 rows: 160 registers, 63.4 us at 131072 keys x 8 heads x 128).
+// fit (with q and p as A, halves stacked in its 16 rows, it took 160 registers and 63.4 us for the first of these, and
+// 60.0 with the codes as A at the same stage). Up to 4 rows put both halves into one operand: 47.7.
 //
 // Dequantising: a code or'ed into the mantissa of an f16 constant, then one HFMA2 with the group's factor and offset
 // gives (n - 8) scale / 16 without rounding (scale_of). Eight codes take 5 integer and 4 HFMA2 instructions. (4-bit

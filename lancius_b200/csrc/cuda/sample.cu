@@ -10,9 +10,13 @@
 // 2^18 tokens fit 62 bits. The draw's sums are FP64 in a fixed order. Weights are FP64: with FP32 ones a drawn token
 // would differ from the exact one in about one row of a thousand.
 //
-// Bound: HBM for large batches (each logit read once), the length of the chain of passes for small ones. A row is
-// spread over a cluster of 1 to 8 CTAs that hold it in shared memory through all passes and exchange histograms and
-// sums through each other's shared memory.
+// k_sample: a row is spread over a cluster of 1 to 8 CTAs that hold it in shared memory through all passes and exchange
+// histograms and sums through each other's shared memory; HBM is read once. Bound by the passes' instructions and by
+// the chain of barriers between them, not by HBM: of 29 us that a cluster needs for a quarter of 50021 logits a CTA with top-p,
+// the load takes 4, the histogram 8, its scan 3, the list 3, the ranking 1, the draw's weights 6, the draw 1.
+// 32000 logits with every filter: 9.9 us; 200 x 50021 with mixed filters: 62.6 us (plain top-p 93, top-k of 50 45).
+// k_sample_open, without filters: one pass, no part of the row kept. 64 x 131072: 20.6 us, of which the loads and
+// barriers alone take 9 (as greedy rows measure them) and the FP64 pipe is busy for 6: 12 instructions a logit.
 #include "lcu_internal.h"
 #include <cooperative_groups.h>
 #include <math.h>
@@ -63,7 +67,9 @@ struct Row {
 };
 
 constexpr int ALL = 0x7fffffff;
-__device__ __forceinline__ bool kept(const Row& r, float x, int i) { return x >= r.tau && (r.last == ALL || x > r.tau || r.first + i <= r.last); }
+__device__ __forceinline__ bool kept(const Row& r, float x, int i) {
+    return x >= r.tau && (r.last == ALL || x > r.tau || r.first + i <= r.last);
+}
 // Calls use(logit, index in the part) for the kept logits of this CTA's part, 4 neighbours at a time per thread. The
 // part is padded with -infinity, which is never kept, to a multiple of BLOCK.
 template <typename Use>
@@ -334,7 +340,9 @@ struct ValueBins {
         per = (BINS - 1) / range;
         return range > 0.f && range < INFINITY && per < 1e30f;
     }
-    __device__ __forceinline__ int operator()(float x) const { return __float_as_int(fminf((max - x) * per, BINS - 1) + 8388608.f) & 0xffff; }   // rounded by adding 2^23
+    __device__ __forceinline__ int operator()(float x) const {   // rounded by adding 2^23
+        return __float_as_int(fminf((max - x) * per, BINS - 1) + 8388608.f) & 0xffff;
+    }
 };
 
 // Moves the row's cut to the rank at which the running count (MASS = false: k) or mass (p times the mass of what is
@@ -588,10 +596,12 @@ __global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ tok
     }
 }
 
-// Without filters: one pass. Each warp takes blocks of 128 logits, whose weights are summed relative to the block's own
-// maximum; the sums are brought to the row's maximum when that is known, and the drawn block's logits are read again.
+// Without filters: one pass. Each warp takes blocks of 256 logits (128: 25.6 us for 64 x 131072, 256: 20.6, 512: the same, and
+// slower rows of 32000), whose weights are summed relative to the block's own maximum; the sums are brought to the
+// row's maximum when that is known, and the drawn block's logits are read again.
 // Nothing of a row stays in shared memory but a maximum and a sum per block, so twice as many CTAs run as above.
-constexpr int OPEN_THREADS = 256, OPEN_WARPS = OPEN_THREADS / 32, OPEN_SUBS = 2, OPEN_BLOCK = OPEN_SUBS * BLOCK, OPEN_MOST = 32768;
+constexpr int OPEN_THREADS = 256, OPEN_WARPS = OPEN_THREADS / 32, OPEN_SUBS = 2, OPEN_BLOCK = OPEN_SUBS * BLOCK;
+constexpr int OPEN_MOST = 32768;   // logits of a CTA
 
 __global__ void __launch_bounds__(OPEN_THREADS, 4) k_sample_open(int32_t* __restrict__ token, const float* __restrict__ logits,
                                                                  size_t ld, int vocab, int part, int vec, const float* temperature,
@@ -742,10 +752,10 @@ __global__ void __launch_bounds__(OPEN_THREADS, 4) k_sample_open(int32_t* __rest
 
 lancius_error bad(lancius_error e) { lancius_set_error(e); return e; }
 
-// CTAs per row. With filters parts of at most 16384 logits, so that two CTAs fit on an SM, without them of 32768; for few
+// CTAs per row. With filters parts of at most 16384 logits, so that two CTAs fit on an SM, without them of OPEN_MOST; for few
 // rows up to 8 with at least 2048, as long as all CTAs run at once.
 int cluster_of(size_t rows, size_t vocab, bool open) {
-    const size_t resident = (open ? 4 : 2) * LCU_SMS, most = open ? 32768 : 16384;
+    const size_t resident = (open ? 4 : 2) * LCU_SMS, most = open ? OPEN_MOST : 16384;
     int c = 1;
     while (c < MAX_CLUSTER && vocab > most * c) c *= 2;
     while (c < MAX_CLUSTER && rows * c * 2 <= resident && vocab >= 4096 * (size_t)c) c *= 2;
