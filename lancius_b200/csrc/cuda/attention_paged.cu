@@ -39,8 +39,11 @@
 // Chunks of a sequence are joined by k_attn_paged_join. Rows past a tile's last visible key are filled with
 // zeros by cp.async, so stale bytes never reach an MMA.
 #include "kv_paged.cuh"
+#include <cooperative_groups.h>
 #include <math.h>
 #include <type_traits>
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -48,6 +51,7 @@ constexpr int WARPS = 4, THREADS = 32 * WARPS, TILE = 32;
 // Keys of a CTA, at most, where all run at once and in rounds. An MMA truncates its sum, and a warp of the CTA adds a
 // fourth of them up in one accumulator.
 constexpr int MAX_CHUNK = 2048, ROUND = 1280;
+constexpr int MAX_CLUSTER = 8;
 constexpr float P_BIAS = 7.f;     // p = 2^(s - m + 7): more of the small weights stay above f16's smallest step
 constexpr uint32_t NONE = 0xffffffffu;
 constexpr float RAISE = 8.f;      // the running maximum moves only when exceeded by 2^8: p <= 2^15 fits f16
@@ -148,9 +152,13 @@ __device__ __forceinline__ void split(float p0, float p1, uint32_t& hi, uint32_t
     lo = as_u32(__floats2half2_rn(p0 - f.x, p1 - f.y));
 }
 
-struct Split { int chunk, splits; };
+struct Split {
+    int chunk, splits;
+    bool cluster;   // k_attn_paged's CLUSTER
+};
 
-template <int D, int ROWS>
+// CLUSTER: the splits of a block of rows are a cluster, whose CTAs join their sums without another kernel
+template <int D, int ROWS, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, Shape<D, ROWS>::RESIDENT)
 k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, bool q_wide, int hq, KvPagesDev p, KvBatchDev b,
              float scale_log2, Split sp, float* __restrict__ part_o, float2* __restrict__ part_ml) {
@@ -160,12 +168,14 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float col_scale[COLS];
     __shared__ float sm_m[WARPS][COLS], sm_l[WARPS][COLS];
+    __shared__ float2 cl_ml[COLS];
     asm volatile("griddepcontrol.launch_dependents;");
 
     const uint32_t zero = (uint32_t)p.heads >> 31;
     const Masks masks{0x000f000fu + zero, 0x00f000f0u + zero};
     const int group = hq / p.heads, blocks = gridDim.x / sp.splits;
-    const int split_id = blockIdx.x / blocks, block = blockIdx.x % blocks, head = blockIdx.y, s = blockIdx.z;
+    const int split_id = CLUSTER ? blockIdx.x % sp.splits : blockIdx.x / blocks;
+    const int block = CLUSTER ? blockIdx.x / sp.splits : blockIdx.x % blocks, head = blockIdx.y, s = blockIdx.z;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     int first, count;
     kv_new_tokens(b, s, first, count);
@@ -175,7 +185,13 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     if (split_id == 0 && block == 0 && tid == 0 && (len > b.max_len || count > b.max_new)) g_attn_paged_fault = 1;
     const int cols = min(COLS, used * group - block * COLS);     // rows of this block
     const int parts = max(1, (keys + sp.chunk - 1) / sp.chunk);   // chunks of this sequence
-    if (cols <= 0 || split_id >= parts) return;
+    if (cols <= 0 || split_id >= parts) {
+        if (CLUSTER && cols > 0 && parts > 1) {   // the others' barriers
+            cg::this_cluster().sync();
+            cg::this_cluster().sync();
+        }
+        return;
+    }
 
     // this thread's R rows of q: 2t, 2t + 1 (and 8 more); packed: 2 (t % 2) and the next, held by t and t ^ 2
     auto row_at = [&](int r) { return PACK ? 2 * (t & 1) + r : 2 * t + (r & 1) + (r >> 1) * 8; };
@@ -619,7 +635,10 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
             acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
         }
         const size_t row = (size_t)(first + ci / group) * hq + head * group + ci % group;
-        if (parts == 1) {
+        if (CLUSTER && parts > 1) {
+            reinterpret_cast<float4*>(smem)[x] = acc;   // q's fragments are done with
+            if (d == 0) cl_ml[c] = make_float2(M, L);
+        } else if (parts == 1) {
             const float inv = L == 0.f ? 0.f : 16.f * p.v_unit / L;   // V comes as value / 16
             float* dst = out + row * D + d;
             dst[0] = acc.x * inv; dst[1] = acc.y * inv; dst[2] = acc.z * inv; dst[3] = acc.w * inv;
@@ -629,6 +648,35 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
             if (d == 0) part_ml[at] = make_float2(M, L);
         }
     }
+    if (!CLUSTER || parts == 1) return;
+    // out row = sum over the chunks of 2^(m - M) o / sum of 2^(m - M) l, the row's channels shared out over the cluster
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    for (int x = split_id * THREADS + tid; x < cols * (D / 4); x += parts * THREADS) {
+        const int c = x / (D / 4), ci = block * COLS + c;
+        float2 ml[MAX_CLUSTER];
+        float4 v[MAX_CLUSTER];
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int r = 0; r < MAX_CLUSTER; r++)
+            if (r < parts) {
+                ml[r] = *cl.map_shared_rank(&cl_ml[c], r);
+                v[r] = *cl.map_shared_rank(reinterpret_cast<float4*>(smem) + x, r);
+                M = fmaxf(M, ml[r].x);
+            }
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int r = 0; r < MAX_CLUSTER; r++)
+            if (r < parts) {
+                const float f = ml[r].x == -INFINITY ? 1.f : ex2(ml[r].x - M);   // a chunk without a visible key holds zeros (or NaN)
+                L += f * ml[r].y;
+                acc.x += f * v[r].x; acc.y += f * v[r].y; acc.z += f * v[r].z; acc.w += f * v[r].w;
+            }
+        const float inv = L == 0.f ? 0.f : 16.f * p.v_unit / L;
+        float* dst = out + ((size_t)(first + ci / group) * hq + head * group + ci % group) * D + x % (D / 4) * 4;
+        dst[0] = acc.x * inv; dst[1] = acc.y * inv; dst[2] = acc.z * inv; dst[3] = acc.w * inv;
+    }
+    cl.sync();   // nobody leaves while its sums are read
 }
 
 // out row = sum over its chunks of 2^(m - M) o / sum of 2^(m - M) l; one CTA of JOIN warps per row, chunk c is warp
@@ -734,6 +782,7 @@ auto with_shape(int D, int rows, F f) {
 // ones cost more starts and joins and long ones an idle end (64 sequences of up to 8000 keys, 8 heads with 8 rows: 146.8 us
 // with 512 keys, 137.4 with 1024, 135.6 with 1280, 135.8 with 1536; 32 of up to 8192, 8 heads with one: 71.0, 69.3, 69.2,
 // 70.6). Sequences of a batch are taken as three quarters of the longest. A multiple of one tile per warp.
+// Up to 8 chunks of up to 8 rows, where all CTAs run at once, join as a cluster (777 keys: 5.0 us in one launch, 5.4 in two).
 Split plan(const KvPagesDev& p, const KvBatchDev& b, int D, int group) {
     const int rows = group * b.max_new;
     const size_t slots = LCU_SMS * with_shape(D, rows, [](auto d, auto n) { return (size_t)Shape<d, n>::RESIDENT; });
@@ -746,7 +795,8 @@ Split plan(const KvPagesDev& p, const KvBatchDev& b, int D, int group) {
     chunk = (chunk + STEP - 1) / STEP * STEP;
     if (chunk < STEP) chunk = STEP;
     if (chunk > most) chunk = most;
-    return Split{(int)chunk, (int)((len + chunk - 1) / chunk)};
+    const size_t splits = (len + chunk - 1) / chunk;
+    return Split{(int)chunk, (int)splits, rows <= 8 && splits > 1 && splits <= MAX_CLUSTER && splits * ctas <= slots};
 }
 size_t part_rows(const KvBatchDev& b, size_t hq, Split sp) { return (size_t)b.n_tokens * hq * sp.splits; }
 
@@ -763,22 +813,37 @@ lancius_error check_call(const lcu_kv_pages* pages, const lcu_kv_batch* batch, s
     return LANCIUS_ERROR_OK;
 }
 
-template <int D, int ROWS>
+template <int D, int ROWS, bool CLUSTER>
 lancius_error launch(float* out, const float* q, size_t q_ld, int hq, const KvPagesDev& p, const KvBatchDev& b, Split sp,
                      float* part_o, float2* part_ml, cudaStream_t st) {
     using S = Shape<D, ROWS>;
     static std::atomic<unsigned long long> allowed{0};   // devices on which the kernel may use its shared memory
-    cudaError_t ce = lcu_allow_smem(allowed, k_attn_paged<D, ROWS>, S::SMEM);
+    auto kernel = k_attn_paged<D, ROWS, CLUSTER>;
+    cudaError_t ce = lcu_allow_smem(allowed, kernel, S::SMEM);
     if (ce != cudaSuccess) return lcu_check_cuda(ce);
     const dim3 grid((unsigned)(sp.splits * row_blocks(D, hq / p.heads * b.max_new)), (unsigned)p.heads, (unsigned)b.n_seqs);
-    k_attn_paged<D, ROWS><<<grid, THREADS, S::SMEM, st>>>(out, q, q_ld, q_ld % 4 == 0 && (uintptr_t)q % 16 == 0, hq, p, b, (float)(1.4426950408889634 / sqrt((double)D)), sp,
-                                                          part_o, part_ml);
-    lcu_note_launch();
-    if (sp.splits == 1) return lcu_launch_status();
-    ce = cudaGetLastError();
-    if (ce != cudaSuccess) return lcu_check_cuda(ce);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at[1];
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = CLUSTER;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = sp.splits;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    ce = cudaLaunchKernelEx(&cfg, kernel, out, q, q_ld, q_ld % 4 == 0 && (uintptr_t)q % 16 == 0, hq, p, b,
+                            (float)(1.4426950408889634 / sqrt((double)D)), sp, part_o, part_ml);
+    if (ce != cudaSuccess) {
+        cudaGetLastError();
+        return lcu_check_cuda(ce);
+    }
+    lcu_note_launch();
+    if (sp.splits == 1 || CLUSTER) return lcu_launch_status();
+    ce = cudaGetLastError();
+    if (ce != cudaSuccess) return lcu_check_cuda(ce);
+    cfg = {};
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // starts while the chunks finish
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3((unsigned)hq, (unsigned)b.max_new, (unsigned)b.n_seqs);
@@ -810,7 +875,7 @@ size_t lcu_attention_paged_workspace(const lcu_kv_pages* pages, const lcu_kv_bat
     KvBatchDev b;
     if (check_call(pages, batch, n_q_heads, &p, &b) != LANCIUS_ERROR_OK || !b.n_seqs || !b.n_tokens || !n_q_heads) return 0;
     const Split sp = plan(p, b, (int)pages->head_dim, (int)(n_q_heads / pages->n_heads));
-    return sp.splits == 1 ? 0 : part_rows(b, n_q_heads, sp) * (pages->head_dim + 2) * sizeof(float);
+    return sp.splits == 1 || sp.cluster ? 0 : part_rows(b, n_q_heads, sp) * (pages->head_dim + 2) * sizeof(float);
 }
 
 lancius_error lcu_attention_paged(float* out, const float* q, size_t q_ld, size_t n_q_heads, const lcu_kv_pages* pages,
@@ -827,7 +892,7 @@ lancius_error lcu_attention_paged(float* out, const float* q, size_t q_ld, size_
     const Split sp = plan(p, b, (int)D, hq / p.heads);
     float* part_o = nullptr;
     float2* part_ml = nullptr;
-    if (sp.splits > 1) {
+    if (sp.splits > 1 && !sp.cluster) {
         const size_t rows = part_rows(b, n_q_heads, sp);
         if (!workspace) return bad(LANCIUS_ERROR_NULL_PTR);
         if ((uintptr_t)workspace & 15u) return bad(LANCIUS_ERROR_UNSUPPORTED_DTYPE);
@@ -837,7 +902,11 @@ lancius_error lcu_attention_paged(float* out, const float* q, size_t q_ld, size_
     }
     cudaStream_t st = lcu_as_stream(stream);
     return with_shape((int)D, hq / p.heads * b.max_new,
-                      [&](auto d, auto n) { return launch<d, n>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st); });
+                      [&](auto d, auto n) {
+                          if constexpr (n <= 8)
+                              if (sp.cluster) return launch<d, n, true>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
+                          return launch<d, n, false>(out, q, q_ld, hq, p, b, sp, part_o, part_ml, st);
+                      });
 }
 
 }  // extern "C"
