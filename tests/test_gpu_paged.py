@@ -309,6 +309,41 @@ def test_attention(lib, dim, page, heads, group, lens, new, unit):
         at += k
 
 
+@pytest.mark.parametrize("dim,page,heads,group,lens,new", [
+    (64, 16, 2, 4, [700, 20, 5], [5, 5, 5]),         # 20 rows to a key head
+    (64, 32, 1, 8, [100, 2500], [3, 6]),             # 24 rows, and 48 in two blocks
+    (128, 16, 2, 4, [333, 64], [5, 2]),
+    (128, 32, 1, 8, [200, 90, 1900], [3, 1, 6]),
+    (128, 64, 3, 3, [130], [9]),                     # 27 rows: blocks of 16 whose second is not full
+    (256, 16, 1, 4, [300, 44], [5, 1]),
+    (256, 32, 2, 8, [1000, 257, 1], None),
+    (128, 16, 8, 4, [777], None),                    # up to eight chunks: joined within one launch
+    (128, 16, 1, 1, [1024, 1, 128, 129, 0, 900], None),
+    (64, 8, 2, 8, [513, 1000], None),
+    (256, 16, 1, 2, [640], [2])])
+def test_attention_aligned_rows(lib, dim, page, heads, group, lens, new):
+    """Rows of q without gaps, more rows to a key head, few chunks; the second sequence starts with the first one's pages."""
+    c = Cache([max(n, 1) for n in lens], heads, dim, page, seed=8)
+    fill_random(c, 9)
+    c.ks[c.unused], c.vs[c.unused] = 0x7f, 0x7f
+    if len(lens) > 1:
+        same = min(lens[0], lens[1]) // page
+        c.table_np[1, :same] = c.table_np[0, :same]
+        c.table.copy_(i32(c.table_np))
+    hq, one = heads * group, new is None
+    new = [1] * len(lens) if one else new
+    q = np.random.default_rng(sum(lens)).standard_normal((sum(new), hq, dim)).astype(np.float32)
+    b = c.batch(lens, None if one else starts(new), max_new=0 if one else max(new))
+    out = attend(lib, c, b, q, hq).reshape(-1, hq, dim)
+    assert lib.lcu_check_stream(None) == 0
+    at = 0
+    for s, (n, k) in enumerate(zip(lens, new)):
+        kk, vv = c.kv(s, n)
+        ref, size = kvref.attention(q[at:at + k], kk, vv, [n - k + 1 + i for i in range(k)])
+        assert np.max(np.abs(out[at:at + k] - ref)) <= tolerance(size, dim, np.abs(vv).max() if n else 1.0, n)
+        at += k
+
+
 def test_attention_extreme_scores(lib):
     """Rows whose scores lie far apart, large and tiny queries, a zero query, equal keys."""
     c = Cache([300], 1, 128, 16)
@@ -683,6 +718,37 @@ def test_captured_split_attention_follows_lengths(lib):
                 ref, size = kvref.attention(q[s:s + 1], k, v, [n[s]])
                 tol = tolerance(size, 128, np.abs(v).max() if n[s] else 1.0, n[s])
                 assert np.max(np.abs(got[s] - ref[0])) <= tol
+    assert lib.lcu_check_stream(side.cuda_stream) == 0
+
+
+def test_captured_cluster_attention_follows_lengths(lib):
+    """As above with few keys, whose chunks join within the one launch and need no workspace."""
+    c = Cache([1000, 1000, 1000], 2, 64, 16, seed=4)
+    fill_random(c, 22)
+    q = np.random.default_rng(5).standard_normal((3, 12, 64)).astype(np.float32)
+    t = torch.from_numpy(q.reshape(3, -1)).cuda()
+    out = torch.zeros((3, 12 * 64), device="cuda")
+    lens = i32([1000, 1000, 1000])
+    b = L.KvBatch(ptr(c.table), c.table.shape[1], ptr(lens), None, 3, 3, 1000, 1)
+    assert lib.lcu_attention_paged_workspace(c.pages, b, 12) == 0
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        call = lambda: lib.lcu_attention_paged(ptr(out), ptr(t), 768, 12, c.pages, b, None, 0, side.cuda_stream)
+        assert call() == 0
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            assert call() == 0
+        for n in ([1000, 300, 129], [1, 1000, 128], [0, 17, 999], [640, 641, 0]):
+            lens.copy_(i32(n))
+            out.fill_(7.0)
+            g.replay()
+            side.synchronize()
+            got = out.view(3, 12, 64).cpu().numpy()
+            for s in range(3):
+                k, v = c.kv(s, n[s])
+                ref, size = kvref.attention(q[s:s + 1], k, v, [n[s]])
+                assert np.max(np.abs(got[s] - ref[0])) <= tolerance(size, 64, np.abs(v).max() if n[s] else 1.0, n[s])
     assert lib.lcu_check_stream(side.cuda_stream) == 0
 
 
