@@ -245,12 +245,20 @@ __global__ void __launch_bounds__(THREADS) k_kv_read(float* __restrict__ k_out, 
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 lancius_error bad(lancius_error e) { lancius_set_error(e); return e; }
 
-// Warps per token, as a power of two: few tokens are spread over about 8 warps per SM (each repeats the sines), as far as
-// there are rows
+// Warps per token, as a power of two: the number with the least rounds of 32 warps per SM times the steps of a warp over its
+// rows, where the start of a warp with its sines counts as 2 steps. Above 8 warps per SM at least 2 steps, whose loads are in
+// flight together. (5380 tokens of 32 + 16 heads of 128: one warp 57.6 us, as they are just over one round, 46.6
+// with four; 2000 tokens 35.3 and 28.4; 128 tokens 4.5 with 2 steps a warp, 5.2 with one.)
 int part_shift(int tokens, int rows, int rows_at_once) {
-    int shift = 0;
-    while (((size_t)tokens << shift) < 8 * LCU_SMS && (rows_at_once << shift) < rows) shift++;
-    return shift;
+    int best = 0;
+    size_t least = SIZE_MAX;
+    for (int shift = 0; shift == 0 || (rows_at_once << (shift - 1)) < rows; shift++) {
+        const size_t warps = (size_t)tokens << shift, at_once = (size_t)rows_at_once << shift;
+        const size_t rounds = (warps + 32 * LCU_SMS - 1) / (32 * LCU_SMS), steps = (rows + at_once - 1) / at_once;
+        if (shift && steps < 2 && warps > 8 * LCU_SMS) break;
+        if (rounds * (steps + 2) < least) { least = rounds * (steps + 2); best = shift; }
+    }
+    return best;
 }
 unsigned part_blocks(int tokens, int shift) { return (unsigned)((((size_t)tokens << shift) + WARPS - 1) / WARPS); }
 // widest access to rows `ld` floats apart (load8, store8)
