@@ -14,7 +14,7 @@
 // histograms and sums through each other's shared memory; HBM is read once. Bound by the passes' instructions and by
 // the chain of barriers between them, not by HBM: of 29 us that a cluster needs for a quarter of 50021 logits a CTA with top-p,
 // the load takes 4, the histogram 8, its scan 3, the list 3, the ranking 1, the draw's weights 6, the draw 1.
-// 32000 logits with every filter: 9.9 us; 200 x 50021 with mixed filters: 62.6 us (plain top-p 93, top-k of 50 45).
+// 32000 logits with every filter: 9.7 us; 200 x 50021 with mixed filters: 56.5 us (top-p alone 84, top-k of 50 alone 40).
 // k_sample_open, without filters: one pass, no part of the row kept. 64 x 131072: 20.6 us, of which the loads and
 // barriers alone take 9 (as greedy rows measure them) and the FP64 pipe is busy for 6: 12 instructions a logit.
 #include "lcu_internal.h"
@@ -45,10 +45,14 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k &
 struct Shared {
     uint32_t low[BINS], high[BINS];    // of a bin: its sum (counts in low alone)
     float warp_max[WARPS], warp_min[WARPS];
-    u64 list[LIST], list_mass[LIST];   // key << 32 | ~index, so that larger means an earlier rank
+    union {
+        u64 list[LIST];   // key << 32 | ~index, so that larger means an earlier rank
+        double block_mass[MAX_BLOCKS];   // of the draw, when the list is done with
+    };
+    u64 list_mass[LIST];
     double power[16];
     u64 warp_sum[WARPS];
-    double block_mass[MAX_BLOCKS], mass_of[MAX_CLUSTER];   // mass_of: written by every CTA of the cluster
+    double mass_of[MAX_CLUSTER];   // mass_of: written by every CTA of the cluster
     float max, min, tau;
     int at, found, bin, last;
     uint32_t listed;
@@ -451,9 +455,13 @@ __device__ __forceinline__ int draw_in_part(double mine, bool mine_any, int per,
     return __shfl_sync(0xffffffffu, block * BLOCK + 4 * lane + drawn, at);
 }
 
-__global__ void __launch_bounds__(THREADS, 2) k_sample(int32_t* __restrict__ token, const float* __restrict__ logits, size_t ld, int vocab,
-                                                    int part, int vec, const float* temperature, const int32_t* top_k,
-                                                    const float* top_p, const float* min_p, const float* u) {
+// RESIDENT CTAs per SM: 3 take 40 registers a thread and some spills, which pays as soon as there are more CTAs than 2 per SM
+// hold (200 x 50021, mixed filters: 56.5 us, 62.8 with 2; one row of 32000: 9.9 and 9.7)
+template <int RESIDENT>
+__global__ void __launch_bounds__(THREADS, RESIDENT) k_sample(int32_t* __restrict__ token, const float* __restrict__ logits, size_t ld,
+                                                              int vocab, int part, int vec, const float* temperature,
+                                                              const int32_t* top_k, const float* top_p, const float* min_p,
+                                                              const float* u) {
     extern __shared__ __align__(16) float part_of_row[];
     __shared__ Shared sh;
     cg::cluster_group cl = cg::this_cluster();
@@ -752,7 +760,7 @@ __global__ void __launch_bounds__(OPEN_THREADS, 4) k_sample_open(int32_t* __rest
 
 lancius_error bad(lancius_error e) { lancius_set_error(e); return e; }
 
-// CTAs per row. With filters parts of at most 16384 logits, so that two CTAs fit on an SM, without them of OPEN_MOST; for few
+// CTAs per row. With filters parts of at most 16384 logits, so that two CTAs fit on an SM (three with 12544), without them of OPEN_MOST; for few
 // rows up to 8 with at least 2048, as long as all CTAs run at once.
 int cluster_of(size_t rows, size_t vocab, bool open) {
     const size_t resident = (open ? 4 : 2) * LCU_SMS, most = open ? OPEN_MOST : 16384;
@@ -788,11 +796,17 @@ extern "C" lancius_error lcu_sample(int32_t* token, const float* logits, size_t 
     if (open) {
         ce = cudaLaunchKernelEx(&cfg, k_sample_open, token, logits, ld, (int)vocab, (int)part, vec, temperature, u);
     } else {
-        static std::atomic<unsigned long long> allowed{0};
-        ce = lcu_allow_smem(allowed, k_sample, (int)(MAX_VOCAB / MAX_CLUSTER * sizeof(float)));
-        if (ce != cudaSuccess) return lcu_check_cuda(ce);
         cfg.dynamicSmemBytes = (part + BLOCK - 1) / BLOCK * BLOCK * sizeof(float);   // whole blocks are read
-        ce = cudaLaunchKernelEx(&cfg, k_sample, token, logits, ld, (int)vocab, (int)part, vec, temperature, top_k, top_p, min_p, u);
+        auto launch = [&](auto kernel, std::atomic<unsigned long long>& allowed, int most) {
+            const cudaError_t e = lcu_allow_smem(allowed, kernel, most);
+            return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, kernel, token, logits, ld, (int)vocab, (int)part, vec, temperature,
+                                                             top_k, top_p, min_p, u);
+        };
+        static std::atomic<unsigned long long> allowed2{0}, allowed3{0};
+        constexpr size_t THIRD = (228 * 1024) / 3 - 1024 - sizeof(Shared);   // of an SM's shared memory
+        ce = rows * c > 2 * LCU_SMS && cfg.dynamicSmemBytes <= THIRD
+                 ? launch(k_sample<3>, allowed3, (int)THIRD)
+                 : launch(k_sample<2>, allowed2, (int)(MAX_VOCAB / MAX_CLUSTER * sizeof(float)));
     }
     if (ce != cudaSuccess) {
         cudaGetLastError();

@@ -460,6 +460,19 @@ def test_sample_rows_differ(lib):
     check_sample(sample(lib, x, u, **kw), x, u, **kw)
 
 
+@pytest.mark.parametrize("rows,vocab", [(400, 1500), (170, 20001)])
+def test_sample_many_rows(lib, rows, vocab):
+    """More CTAs than two per SM."""
+    rng = np.random.default_rng(vocab)
+    x = (rng.standard_normal((rows, vocab)) * rng.uniform(0.5, 4, (rows, 1))).astype(np.float32)
+    x[::3] = torch.from_numpy(x[::3]).bfloat16().float().numpy()
+    kw = dict(temperature=np.where(rng.random(rows) < 0.1, 0, rng.random(rows) + 0.3), top_k=rng.integers(-200, 700, rows),
+              top_p=rng.random(rows) * 1.5, min_p=rng.random(rows) * 0.1 - 0.06)
+    u = rng.random(rows)
+    check_sample(sample(lib, x, u, **kw), x, u, **kw)
+    check_sample(sample(lib, x, u), x, u)
+
+
 def test_sample_odd_logits(lib):
     inf, nan = np.inf, np.nan
     v = 300
