@@ -10,7 +10,7 @@
 // tensor pipe is busy for 21 and 38 %. Four warps a quarter of an SM issue them at nine tenths of the rate within the
 // loop, at 61 % over the kernel, as a CTA spends a quarter of its time on lengths, first loads and its merge. MMAs
 // do not overlap with the half-rate LOP3 and HFMA2 (18.3 clocks for a group with its MMA, 9.5 without).
-//   131072 keys of one sequence, 8 key heads of 128, 4 rows each: 40.7 us, 3.7 TB/s (0.57 of the measured copy rate)
+//   131072 keys of one sequence, 8 key heads of 128, 4 rows each: 41.0 us, 3.7 TB/s (0.56 of the measured copy rate)
 //   32 sequences of up to 8192 keys, 8 key heads of 128, one row each: 66.4 us, 3.55 TB/s (0.54)
 //   64 sequences of up to 8000 keys, 8 key heads of 128, 8 rows each: 133 us, 3.4 TB/s (0.51); the loads alone 83 us
 //   24 sequences of up to 3001 keys, 4 key heads of 64, 20 rows each: 19.5 us
