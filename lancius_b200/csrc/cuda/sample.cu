@@ -14,7 +14,7 @@
 // histograms and sums through each other's shared memory; HBM is read once. Bound by the passes' instructions and by
 // the chain of barriers between them, not by HBM: of 29 us that a cluster needs for a quarter of 50021 logits a CTA with top-p,
 // the load takes 4, the histogram 8, its scan 3, the list 3, the ranking 1, the draw's weights 6, the draw 1.
-// 32000 logits with every filter: 9.7 us; 200 x 50021 with mixed filters: 56.5 us (top-p alone 84, top-k of 50 alone 40).
+// 32000 logits with every filter: 8.3 us; 200 x 50021 with mixed filters: 55.3 us (top-p alone 84, top-k of 50 alone 34).
 // k_sample_open, without filters: one pass, no part of the row kept. 64 x 131072: 20.6 us, of which the loads and
 // barriers alone take 9 (as greedy rows measure them) and the FP64 pipe is busy for 6: 12 instructions a logit.
 #include "lcu_internal.h"
@@ -139,7 +139,7 @@ struct Found {
     int bin;
     u64 before, in_bin, total;   // sum before the bin, in it, of all bins
 };
-template <bool MASS, typename Bin, typename Target>
+template <bool MASS, bool FEW, typename Bin, typename Target>
 __device__ Found find_bin(cg::cluster_group& cl, Shared& sh, Row& r, u64 before, Bin bin_of, Target target_of) {
     const int tid = threadIdx.x, lane = tid & 31, ranks = cl.num_blocks(), rank = cl.block_rank(), slice = BINS / ranks;
     if (!r.fresh) {
@@ -161,6 +161,21 @@ __device__ Found find_bin(cg::cluster_group& cl, Shared& sh, Row& r, u64 before,
         }
     });
     cl.sync();
+    if (FEW) {   // each CTA adds up and scans the first THREADS bins by itself: two barriers of the cluster less
+        u64 here = 0, x[MAX_CLUSTER];
+#pragma unroll
+        for (int c = 0; c < MAX_CLUSTER; c++) x[c] = c < ranks ? cl.map_shared_rank(&sh, min(c, ranks - 1))->low[tid] : 0;
+#pragma unroll
+        for (int c = 0; c < MAX_CLUSTER; c++) here += x[c];
+        const u64 upto = block_scan(sh, here);
+        if (tid == THREADS - 1) { sh.slice_sum = upto; sh.found = 0; }
+        __syncthreads();
+        const u64 total = sh.slice_sum, at = before + upto - here;
+        const double target = target_of(total);
+        if ((double)at < target && (double)(at + here) >= target) { sh.bin = tid; sh.before = at; sh.in_bin = here; sh.found = 1; }
+        __syncthreads();
+        return Found{sh.found != 0, sh.bin, sh.before, sh.in_bin, total};
+    }
     // each CTA adds up its slice of the bins over the cluster and scans it, q neighbours a thread
     const int b0 = rank * slice, q = max(1, slice / THREADS);
     constexpr int PER = BINS / THREADS;
@@ -337,15 +352,16 @@ __device__ void finish_ties(cg::cluster_group& cl, Shared& sh, Row& r, float val
 
 // Bins of equal width in the logit, down to weights of 2^-144; false where the logits' range allows none.
 struct ValueBins {
-    float max, per;
-    __device__ bool make(const Row& r) {
+    float max, per, most;
+    __device__ bool make(const Row& r, int bins) {
+        most = (float)(bins - 1);
         const float range = fminf(r.max - r.min, 144.f * 16 / (float)r.rate);
         max = r.max;
-        per = (BINS - 1) / range;
+        per = most / range;
         return range > 0.f && range < INFINITY && per < 1e30f;
     }
     __device__ __forceinline__ int operator()(float x) const {   // rounded by adding 2^23
-        return __float_as_int(fminf((max - x) * per, BINS - 1) + 8388608.f) & 0xffff;
+        return __float_as_int(fminf((max - x) * per, most) + 8388608.f) & 0xffff;
     }
 };
 
@@ -354,9 +370,13 @@ struct ValueBins {
 template <bool MASS>
 __device__ bool cut(cg::cluster_group& cl, Shared& sh, Row& r, int k, double p, double u, int32_t* token) {
     auto first_target = [&](u64 total) { return MASS ? fmax(p * (double)total, 0.5) : (double)k; };
+    // The upper few thousand logits lie apart: fewer bins hold no more than a list of them each, and one pass less over
+    // the cluster finds the bin (32000 logits, top-k of 50: 8.9 us, with 2048 bins 10.2).
+    const bool few = !MASS && k <= 4096;
     ValueBins bin_of;
-    if (bin_of.make(r)) {
-        const Found f = find_bin<MASS>(cl, sh, r, 0, bin_of, first_target);
+    if (bin_of.make(r, few ? THREADS : BINS)) {
+        const Found f = few ? find_bin<MASS, !MASS>(cl, sh, r, 0, bin_of, first_target)
+                            : find_bin<MASS, false>(cl, sh, r, 0, bin_of, first_target);
         const int bin = f.any ? f.bin : BINS;
         if (!MASS && (f.any ? f.before + f.in_bin : f.total) <= SMALL) {
             finish_small(cl, sh, r, k, p, u, token, [&](float x) { return bin_of(x) <= bin; });
@@ -376,7 +396,7 @@ __device__ bool cut(cg::cluster_group& cl, Shared& sh, Row& r, int k, double p, 
             const uint32_t key = key_of(x);
             return key < lo || key > hi ? -1 : (int)((hi - key) >> bits);
         };
-        const Found f = find_bin<MASS>(cl, sh, r, before, key_bin, [&](u64 total) { return first ? first_target(total) : target; });
+        const Found f = find_bin<MASS, false>(cl, sh, r, before, key_bin, [&](u64 total) { return first ? first_target(total) : target; });
         if (!f.any) return false;
         if (first) target = first_target(f.total);
         before = f.before;
@@ -456,7 +476,7 @@ __device__ __forceinline__ int draw_in_part(double mine, bool mine_any, int per,
 }
 
 // RESIDENT CTAs per SM: 3 take 40 registers a thread and some spills, which pays as soon as there are more CTAs than 2 per SM
-// hold (200 x 50021, mixed filters: 56.5 us, 62.8 with 2; one row of 32000: 9.9 and 9.7)
+// hold (200 x 50021, mixed filters: 56.5 us, with 2 62.8; one row of 32000: 9.9 and 9.7)
 template <int RESIDENT>
 __global__ void __launch_bounds__(THREADS, RESIDENT) k_sample(int32_t* __restrict__ token, const float* __restrict__ logits, size_t ld,
                                                               int vocab, int part, int vec, const float* temperature,
