@@ -36,7 +36,7 @@
 // Work: CTA = (chunk of keys, key head, sequence, block of rows), 4 warps that each take every fourth tile of 32
 // keys through a ring of cp.async stages of their own (no block barrier in the loop) and are merged at the end.
 // Shared-memory rows are swizzled in 16-byte pieces so that both fragment reads are free of bank conflicts.
-// Chunks of a sequence are joined by k_attn_paged_join. Rows past a tile's last visible key are filled with
+// Chunks of a sequence are joined by k_attn_paged_join or, where they are few, by their cluster. Rows past a tile's last visible key are filled with
 // zeros by cp.async, so stale bytes never reach an MMA.
 #include "kv_paged.cuh"
 #include <cooperative_groups.h>
@@ -214,7 +214,8 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 #pragma unroll
     for (int k = 0; k < QC; k++) {
         const int c = q_col(k), ci = block * COLS + c;
-        const float* from = q + (size_t)(first + ci / group) * q_ld + (size_t)(head * group + ci % group) * D + q_owner * (D / 4) + q_octet * 8;
+        const float* from = q + (size_t)(first + ci / group) * q_ld + (size_t)(head * group + ci % group) * D + q_owner * (D / 4) +
+                            q_octet * 8;
 #pragma unroll
         for (int i = 0; i < 8; i++) qx[k][i] = 0.f;
         if (c < cols && q_wide) {
