@@ -278,8 +278,8 @@ lancius_error lcu_kv_read_paged(float* k_out, float* v_out, const lcu_kv_pages* 
 /* out[t][h] = softmax(q[t][h] . K / sqrt(head_dim)) V over keys 0 .. position of row t; query
  * head h reads key head h / (n_q_heads / n_heads). q rows q_ld floats apart, out
  * [n_tokens][n_q_heads * head_dim]. workspace: lcu_attention_paged_workspace() bytes (0 where
- * the keys are few), 16-byte aligned, used by this call alone until it has run (two captured graphs that may run at the
- * same time need two). A NaN or infinity in the cache shows only in the rows that see it: a
+ * the keys are few), 16-byte aligned, used by this call alone until it has run (two captured
+ * graphs that may run at the same time need two). A NaN or infinity in the cache shows only in the rows that see it: a
  * row that sees one in a value is NaN in all its channels. Pages outside the cache count as zeros; they, and
  * lengths over max_seq_len or max_new, are reported as above (the keys and rows over the
  * bound are left out). */

@@ -36,8 +36,8 @@
 // Work: CTA = (chunk of keys, key head, sequence, block of rows), 4 warps that each take every fourth tile of 32
 // keys through a ring of cp.async stages of their own (no block barrier in the loop) and are merged at the end.
 // Shared-memory rows are swizzled in 16-byte pieces so that both fragment reads are free of bank conflicts.
-// Chunks of a sequence are joined by k_attn_paged_join or, where they are few, by their cluster. Rows past a tile's last visible key are filled with
-// zeros by cp.async, so stale bytes never reach an MMA.
+// Chunks of a sequence are joined by k_attn_paged_join or, where they are few, by their cluster. Rows past a tile's last
+// visible key are filled with zeros by cp.async, so stale bytes never reach an MMA.
 #include "kv_paged.cuh"
 #include <cooperative_groups.h>
 #include <math.h>
