@@ -81,7 +81,7 @@ def kept(x, temperature, top_k, top_p, min_p):
     if top_k > 0:
         keep &= rank < top_k
     if min_p > 0:
-        keep &= (ws >= min_p) | (rank == 0)
+        keep &= ws >= min(min_p, 1.0)
     mass = np.cumsum(np.where(keep, ws, 0.0))
     if top_p < 1:
         keep &= (np.concatenate(([0.0], mass[:-1])) < top_p * mass[-1]) | (rank == 0)

@@ -501,6 +501,18 @@ def test_sample_odd_logits(lib):
     assert sample(lib, x, 0.1)[[0, 3]].tolist() == [-1, -1]
 
 
+def test_sample_min_p_over_one(lib):
+    """Counts as 1: all that equal the largest stay."""
+    x = np.zeros((3, 40), np.float32)
+    x[1, 5:30] = 2.0
+    x[2, [3, 39]] = np.inf
+    for u in (0.0, 0.3, 0.6, 0.999):
+        uu = np.full(3, u, np.float32)
+        got = sample(lib, x, uu, min_p=1.3)
+        check_sample(got, x, uu, min_p=1.0)
+        assert got.tolist() == [int(40 * u), 5 + int(25 * u), 39 if u >= 0.5 else 3]
+
+
 def test_sample_extreme_temperatures(lib):
     """Temperatures at which every other logit weighs nothing, or all weigh the same; logits far from zero."""
     rng = np.random.default_rng(11)
