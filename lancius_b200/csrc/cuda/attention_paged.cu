@@ -55,6 +55,9 @@ constexpr int MAX_CLUSTER = 8;
 constexpr float P_BIAS = 7.f;     // p = 2^(s - m + 7): more of the small weights stay above f16's smallest step
 constexpr uint32_t NONE = 0xffffffffu;
 constexpr float RAISE = 8.f;      // the running maximum moves only when exceeded by 2^8: p <= 2^15 fits f16
+// From here on a score may lie 1/4 and more from its FP32 number, and a maximum held in FP32 that far from the score it
+// came from: scores are rounded before the maximum is taken off, so that the largest is 0 and not some 2^n.
+constexpr float FAR = 4194304.f;
 
 __device__ int g_attn_paged_fault = 0;
 
@@ -340,6 +343,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     constexpr int VG = D == 256 ? 2 : 1;   // groups of a thread's channels of V
     const int vs_at = 2 * S::CODES + S::SCALES + 2 * t * S::SROW + (D == 64 ? g >> 1 : g * VG);
     int stage = 0, stage_in = (S::STAGES - 1) * S::STAGE;
+    bool far = false;   // some running maximum of the warp is at least FAR
 
     for (int i = 0; i < tiles; i++) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2));
@@ -498,6 +502,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
         }
         if (__any_sync(0xffffffffu, raise)) {   // some key exceeds its row's maximum by enough
             float f[R];
+            far = false;
 #pragma unroll
             for (int r = 0; r < R; r++) {
 #pragma unroll
@@ -506,7 +511,9 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
                 f[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - mx);   // nothing was summed before the first key
                 m[r] = mx;
                 l[r] *= f[r];
+                far = far || (fabsf(mx) >= FAR && mx > -INFINITY);
             }
+            far = __any_sync(0xffffffffu, far);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -525,12 +532,15 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 #pragma unroll
                 for (int x = 0; x < X; x++) pw[u][x] = ex2(fmaf(sv[r][x], cs[r], -base));
             }
-            if (poison) {
+            if (poison || far) {
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int x = 0; x < X; x++)
-                        if ((poison >> (key1 - key0 + 8 * x) & 1) && key1 + 8 * x < limit[2 * nt + u]) pw[u][x] = NAN;
+                    for (int x = 0; x < X; x++) {
+                        const int r = 2 * nt + u;
+                        if (far) pw[u][x] = ex2(__fsub_rn(__fmul_rn(sv[r][x], cs[r]), m[r] == -INFINITY ? 0.f : m[r]) + P_BIAS);
+                        if ((poison >> (key1 - key0 + 8 * x) & 1) && key1 + 8 * x < limit[r]) pw[u][x] = NAN;
+                    }
             }
 #pragma unroll
             for (int u = 0; u < 2; u++)

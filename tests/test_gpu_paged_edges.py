@@ -1,0 +1,42 @@
+"""The paged cache, its attention and the sampler where numbers, lengths and bounds end: units and queries whose product
+leaves FP32's range, token ranges that do not fit, weights far below the largest, the longest sequences, prompts."""
+import numpy as np
+import pytest
+
+import kvref
+from test_gpu_paged import Cache, attend, fill_random, lib, tolerance  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+# ---- attention: units ------------------------------------------------------------------------------------------
+
+def check_scores(lib, dim, group, unit, top):
+    """Keys in multiples of `unit`, queries of up to `top`, lengths that leave masked keys in the last tile."""
+    lens = [777, 33]
+    c = Cache(lens, 1, dim, 16, (unit, 1.0), seed=1)
+    fill_random(c, dim)
+    rng = np.random.default_rng(dim + group)
+    q = rng.standard_normal((2, group, dim)).astype(np.float32)
+    q = (q / np.abs(q).max() * top).astype(np.float32)
+    out = attend(lib, c, c.batch(lens), q, group).reshape(2, group, dim)
+    for s, n in enumerate(lens):
+        k, v = c.kv(s, n)
+        ref, size = kvref.attention(q[s:s + 1], k, v, [n])
+        if size < 1e6:
+            tol = tolerance(size, dim, np.abs(v).max(), n)
+        else:   # scores next to each other differ by far more than their rounding: one weight, held in 22 bits, a
+            # truncated sum of its halves and two roundings: 2^-22 + 2^-23 + 2^-23
+            x = np.sort(np.einsum("gd,kd->gk", q[s].astype(np.float64), k[:, 0]) / np.sqrt(dim), 1)
+            assert np.all(x[:, -1] - x[:, -2] > max(30, 2.0 ** -17 * size))   # the oracle's
+            tol = 2.0 ** -21 * np.abs(v).max()
+        assert np.max(np.abs(out[s] - ref[0])) <= tol
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("group", [1, 5, 12])
+@pytest.mark.parametrize("top", [1e6, 1e7, 1e8, 1e9, 1e15, 1e30])
+def test_attention_far_scores(lib, dim, group, top):
+    """Scores whose neighbouring FP32 numbers are further apart than the weights reach: one key takes all the weight."""
+    check_scores(lib, dim, group, 1.0, top)
