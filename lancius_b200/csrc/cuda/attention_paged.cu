@@ -155,6 +155,12 @@ __device__ __forceinline__ void split(float p0, float p1, uint32_t& hi, uint32_t
     lo = as_u32(__floats2half2_rn(p0 - f.x, p1 - f.y));
 }
 
+// 16 log2(e) / sqrt(D) * k_unit = factor * 2^exponent, as its product with a row's power of two may leave FP32's range
+struct Scores {
+    float factor;   // 0.5 .. 1
+    int exponent;
+};
+
 struct Split {
     int chunk, splits;
     bool cluster;   // k_attn_paged's CLUSTER
@@ -164,7 +170,7 @@ struct Split {
 template <int D, int ROWS, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, Shape<D, ROWS>::RESIDENT)
 k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, bool q_wide, int hq, KvPagesDev p, KvBatchDev b,
-             float scale_log2, Split sp, float* __restrict__ part_o, float2* __restrict__ part_ml) {
+             Scores scores, Split sp, float* __restrict__ part_o, float2* __restrict__ part_ml) {
     using S = Shape<D, ROWS>;
     constexpr int COLS = ROWS, NT = S::NT, R = 2 * NT;
     constexpr bool PACK = S::PACK;
@@ -301,9 +307,13 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
         int e = (int)(__float_as_uint(amax) >> 23) - 127;          // 2^e <= amax < 2^(e + 1)
         if (amax == 0.f || e > 127) e = 0;
         e = min(max(e, -126), 126);
-        const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
         if (c >= COLS) continue;
-        if (lane % LANES == 0) col_scale[c] = scale_log2 * 16.f * p.k_unit * up;   // K comes as value / 16
+        // K comes as value / 16. Sums of products lie below 2^18 and are multiples of 2^-37: with a scale of 2^100 the
+        // largest takes all the weight, as with any larger scale, and stays finite; with 2^-126 all weigh the same. The scale
+        // is never 0, which would make NaN of a masked score.
+        if (lane % LANES == 0)
+            col_scale[c] = scores.factor * __uint_as_float((uint32_t)(127 + min(max(e + scores.exponent, -125), 100)) << 23);
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             uint4 f;
@@ -538,7 +548,8 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 #pragma unroll
                     for (int x = 0; x < X; x++) {
                         const int r = 2 * nt + u;
-                        if (far) pw[u][x] = ex2(__fsub_rn(__fmul_rn(sv[r][x], cs[r]), m[r] == -INFINITY ? 0.f : m[r]) + P_BIAS);
+                        const float top = m[r] == -INFINITY ? 0.f : m[r];
+                        if (far) pw[u][x] = ex2(__fsub_rn(__fmul_rn(sv[r][x], cs[r]), top) + P_BIAS);
                         if ((poison >> (key1 - key0 + 8 * x) & 1) && key1 + 8 * x < limit[r]) pw[u][x] = NAN;
                     }
             }
@@ -844,8 +855,10 @@ lancius_error launch(float* out, const float* q, size_t q_ld, int hq, const KvPa
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = sp.splits;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    Scores scores;
+    scores.factor = (float)frexp(16 * 1.4426950408889634 / sqrt((double)D) * p.k_unit, &scores.exponent);
     ce = cudaLaunchKernelEx(&cfg, kernel, out, q, q_ld, q_ld % 4 == 0 && (uintptr_t)q % 16 == 0, hq, p, b,
-                            (float)(1.4426950408889634 / sqrt((double)D)), sp, part_o, part_ml);
+                            scores, sp, part_o, part_ml);
     if (ce != cudaSuccess) {
         cudaGetLastError();
         return lcu_check_cuda(ce);

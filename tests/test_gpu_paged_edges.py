@@ -40,3 +40,14 @@ def check_scores(lib, dim, group, unit, top):
 def test_attention_far_scores(lib, dim, group, top):
     """Scores whose neighbouring FP32 numbers are further apart than the weights reach: one key takes all the weight."""
     check_scores(lib, dim, group, 1.0, top)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("group", [1, 5, 12])
+@pytest.mark.parametrize("unit,top", [
+    (1e-20, 1e-27), (1e-30, 1e-38),      # scores next to nothing: the mean of the values
+    (3e37, 2e-38), (1e-38, 1e37),        # large and small numbers with ordinary products
+    (2.0, 1.6e38), (3e37, 1e30)])        # scores past FP32's largest: one key takes all the weight
+def test_attention_scores_scale(lib, dim, group, unit, top):
+    """Keys of any positive unit, queries of any size."""
+    check_scores(lib, dim, group, unit, top)
