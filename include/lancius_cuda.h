@@ -246,7 +246,9 @@ typedef struct {
  * The step's tokens are rows token_start[b] .. token_start[b + 1] - 1 of q, k, v and out, in
  * order, and are the last of the sequence: row token_start[b] + i has position
  * seq_len[b] - n + i. Rows at and after token_start[n_seqs] belong to no sequence and are
- * left as they were, as is the cache for them. A token whose position is negative (an idle
+ * left as they were, as is the cache for them. Rows that token_start places before row 0 or at and
+ * after n_tokens do not exist: they are left out, which lcu_check_stream then reports as
+ * LANCIUS_ERROR_SHAPE_MISMATCH, and the sequence's other rows keep their positions. A token whose position is negative (an idle
  * slot with seq_len 0) is not appended, and its attention row is zero. */
 typedef struct {
     const int32_t* page_table;    /* device, [n_seqs][table_width] */

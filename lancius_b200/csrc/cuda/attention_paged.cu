@@ -186,12 +186,12 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     const int split_id = CLUSTER ? blockIdx.x % sp.splits : blockIdx.x / blocks;
     const int block = CLUSTER ? blockIdx.x / sp.splits : blockIdx.x % blocks, head = blockIdx.y, s = blockIdx.z;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    int first, count;
-    kv_new_tokens(b, s, first, count);
+    int first, count, behind;
+    const bool whole = kv_new_tokens(b, s, first, count, behind);
     const int len = b.seq_len[s];
     const int used = count < b.max_new ? count : b.max_new;       // rows that are computed
     const int keys = min(max(len, 0), b.max_len);
-    if (split_id == 0 && block == 0 && tid == 0 && (len > b.max_len || count > b.max_new)) g_attn_paged_fault = 1;
+    if (split_id == 0 && block == 0 && tid == 0 && (len > b.max_len || count > b.max_new || !whole)) g_attn_paged_fault = 1;
     const int cols = min(COLS, used * group - block * COLS);     // rows of this block
     const int parts = max(1, (keys + sp.chunk - 1) / sp.chunk);   // chunks of this sequence
     if (cols <= 0 || split_id >= parts) {
@@ -205,9 +205,10 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     // this thread's R rows of q: 2t, 2t + 1 (and 8 more); packed: 2 (t % 2) and the next, held by t and t ^ 2
     auto row_at = [&](int r) { return PACK ? 2 * (t & 1) + r : 2 * t + (r & 1) + (r >> 1) * 8; };
     // keys that row c of the block sees: those up to its token's position
+    const int seen = len - count - behind + 1;
     auto limit_of = [&](int c) {
         const int i = (block * COLS + c) / group;
-        return c < cols ? min(len - (count - i) + 1, b.max_len) : 0;
+        return c < cols ? min(seen + i, b.max_len) : 0;
     };
     int limit[R], least = 0x7fffffff;
 #pragma unroll
@@ -712,8 +713,8 @@ __global__ void __launch_bounds__(32 * JOIN) k_attn_paged_join(float* __restrict
     __shared__ float sm_l[JOIN];
     __shared__ __align__(16) float sm_o[JOIN][D];
     const int s = blockIdx.z, i = blockIdx.y, h = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int first, count;
-    kv_new_tokens(b, s, first, count);
+    int first, count, behind;
+    kv_new_tokens(b, s, first, count, behind);
     const int keys = min(max(b.seq_len[s], 0), b.max_len), parts = (keys + sp.chunk - 1) / sp.chunk;
     asm volatile("griddepcontrol.wait;" ::: "memory");   // also before an early return: the next kernel waits for this one only
     if (i >= count || parts <= 1) return;

@@ -45,12 +45,14 @@ __device__ __forceinline__ Place find_place(const KvPagesDev& p, const KvBatchDe
         s = at.any && at.token < b.n_seqs ? at.token : -1;
         end = s + 1;
     } else {   // the last sequence that starts at or before the token holds it, unless it has ended
-        int before = 0;
+        int before = 0, from = 0, to = 0;
+        if (id == 0) { from = b.start[0]; to = b.start[b.n_seqs]; }
 #pragma unroll 4
         for (int i0 = 0; i0 < b.n_seqs; i0 += 32) {
             const int i = i0 + lane;
             before += __popc(__ballot_sync(0xffffffffu, i < b.n_seqs && b.start[i] <= at.token));
         }
+        if (from < 0 || to > b.n_tokens) g_kv_fault = 1;   // rows outside the arrays
         end = b.start[before];
         if (before > 0 && at.any && at.token < end) s = before - 1;
     }

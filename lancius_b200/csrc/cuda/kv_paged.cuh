@@ -17,13 +17,16 @@ struct KvBatchDev {
 // Checks both descriptions and fills the device forms (max_len, max_new resolved).
 lancius_error lcu_kv_describe(const lcu_kv_pages* pages, const lcu_kv_batch* batch, KvPagesDev* p, KvBatchDev* b);
 
-// First row and number of new tokens of sequence s, clipped to the token arrays.
-__device__ __forceinline__ void kv_new_tokens(const KvBatchDev& b, int s, int& first, int& count) {
+// First row and number of new tokens of sequence s, clipped to the token arrays, and the rows that the clipping left out
+// behind them: row first + i has position seq_len[s] - count - behind + i. False: some rows are not in the arrays.
+__device__ __forceinline__ bool kv_new_tokens(const KvBatchDev& b, int s, int& first, int& count, int& behind) {
     first = b.start ? b.start[s] : s;
-    int end = b.start ? b.start[s + 1] : s + 1;
-    if (first < 0) first = 0;
-    if (end > b.n_tokens) end = b.n_tokens;
+    const int last = b.start ? b.start[s + 1] : s + 1, end = min(last, b.n_tokens), from = max(first, 0);
+    const bool whole = first == from && last == end;
+    first = from;
     count = end > first ? end - first : 0;
+    behind = last - end;
+    return whole;
 }
 
 // Index of a cache row in units of rows ([page][head][slot]), or -1 when the position or its

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import kvref
-from test_gpu_paged import Cache, attend, fill_random, lib, tolerance  # noqa: F401
+from test_gpu_paged import BASE, SHAPE, Cache, append, attend, fill_random, lib, ptr, tolerance  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -51,3 +51,41 @@ def test_attention_far_scores(lib, dim, group, top):
 def test_attention_scores_scale(lib, dim, group, unit, top):
     """Keys of any positive unit, queries of any size."""
     check_scores(lib, dim, group, unit, top)
+
+
+# ---- token ranges ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("start,tokens,reported", [
+    ([0, 3, 8], 6, True),        # the second sequence's last two rows are not in the arrays
+    ([0, 3, 8], 3, True),        # nor any of its rows
+    ([-2, 3, 6], 6, True),       # the first one's first two
+    ([1, 3, 6], 8, False)])      # rows of no sequence before and behind
+def test_token_ranges_past_the_arrays(lib, start, tokens, reported):
+    """Rows that the arrays hold have the positions that token_start gives them, in all three calls; the others are reported."""
+    hq, heads, dim, lens = 2, 1, 64, [40, 50]
+    want = SHAPE if reported else 0
+    rows = [(s, t, lens[s] - start[s + 1] + t) for s in range(2) for t in range(max(start[s], 0), min(start[s + 1], tokens))]
+    rng = np.random.default_rng(1)
+    x = rng.standard_normal((tokens, hq + 2 * heads, dim)).astype(np.float32)
+    c = Cache(lens, heads, dim, 16, seed=2)
+    fill_random(c, 3)
+    b = c.batch(lens, start, tokens=tokens, max_new=5)
+    q = append(lib, c, b, x.reshape(tokens, -1), hq).reshape(tokens, hq, dim)
+    assert lib.lcu_check_stream(None) == want and lib.lcu_check_stream(None) == 0
+    ko, vo = torch.full((tokens, heads, dim), 7.0, device="cuda"), torch.full((tokens, heads, dim), 7.0, device="cuda")
+    assert lib.lcu_kv_read_paged(ptr(ko), ptr(vo), c.pages, b, None) == 0
+    assert lib.lcu_check_stream(None) == want
+    out = attend(lib, c, b, x[:, :hq], hq).reshape(tokens, hq, dim)
+    assert lib.lcu_check_stream(None) == want and lib.lcu_check_stream(None) == 0
+    held = set()
+    for s, t, pos in rows:
+        held.add(t)
+        k, v = c.kv(s, lens[s])
+        ref = kvref.rotate(x[t:t + 1, :hq], [pos], BASE)[0]
+        assert np.all(np.abs(q[t] - ref) <= 2.0 ** -23 * np.abs(x[t, :hq]).max())
+        assert np.array_equal(v[pos], kvref.values(*kvref.quantise(x[t, hq + heads:])))
+        assert np.array_equal(vo[t].cpu().numpy(), v[pos].astype(np.float32))
+        ref, size = kvref.attention(x[t:t + 1, :hq], k, v, [pos + 1])
+        assert np.max(np.abs(out[t] - ref[0])) <= tolerance(size, dim, np.abs(v).max(), pos + 1)
+    for t in set(range(tokens)) - held:
+        assert (q[t] == 7.0).all() and (out[t] == 7.0).all() and (ko[t] == 7.0).all()
