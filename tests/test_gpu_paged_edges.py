@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import kvref
-from test_gpu_paged import BASE, SHAPE, Cache, append, attend, fill_random, lib, ptr, tolerance  # noqa: F401
+from test_gpu_paged import BASE, SHAPE, Cache, append, attend, check_sample, fill_random, lib, ptr, sample, tolerance  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -89,3 +89,19 @@ def test_token_ranges_past_the_arrays(lib, start, tokens, reported):
         assert np.max(np.abs(out[t] - ref[0])) <= tolerance(size, dim, np.abs(v).max(), pos + 1)
     for t in set(range(tokens)) - held:
         assert (q[t] == 7.0).all() and (out[t] == 7.0).all() and (ko[t] == 7.0).all()
+
+
+# ---- sampling ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("t", [4e35, 5e35, 7e35, 9e35, 2e36, 3e38])
+def test_sample_hot_rows_of_far_logits(lib, t):
+    """Temperatures at which 693 t is at, or past, FP32's largest number, with logits over all of its range."""
+    rng = np.random.default_rng(13)
+    x = rng.uniform(-3.4e38, 3.4e38, (6, 5003)).astype(np.float32)
+    x[1] = rng.choice(np.array([3.4e38, -3.4e38], np.float32), 5003)
+    x[2] = -3.4e38
+    x[2, [17, 4000]] = 3.4e38
+    x[3, ::2] = -np.inf
+    u = np.array([0.2, 0.4, 0.6, 0.8, 0.3, 0.999], np.float32)
+    for kw in (dict(), dict(top_k=3), dict(top_p=0.7), dict(min_p=0.2)):
+        check_sample(sample(lib, x, u, temperature=t, **kw), x, u, temperature=t, **kw)
