@@ -661,10 +661,10 @@ __global__ void __launch_bounds__(OPEN_THREADS, 4) k_sample_open(int32_t* __rest
             }
         }
     };
-    const float reach = 693.f * t;   // 2^-1000, rounded up where it is subtracted
+    const float reach = 693.14718f * t;   // to 2^-1000, rounded up where it is subtracted
     constexpr float LOWEST = -3.4028235e38f;
     // In two steps, as logits may be further apart than FP32 reaches; from where one of them is infinite they are not.
-    const float half_reach = 346.5f * t;
+    const float half_reach = 346.57359f * t;
     auto nothing_below = [&](float top) { return fmaxf(__fsub_ru(__fsub_ru(top, half_reach), half_reach), LOWEST); };
     // Weights relative to top, the largest or infinite: then the infinite ones share the mass. What lies below `nothing`
     // weighs as much as that, or with to_zero 0.

@@ -93,6 +93,16 @@ def test_token_ranges_past_the_arrays(lib, start, tokens, reported):
 
 # ---- sampling ----------------------------------------------------------------------------------------------------
 
+def test_sample_cut_at_2_to_the_minus_1000(lib):
+    """Without filters and with one: a logit above 2^-1000 of the largest has a weight, one below has none."""
+    t = np.array([0.5, 1.0, 3.0, 0.5, 1.0, 3.0], np.float32)
+    x = np.full((6, 700), -np.inf, np.float32)
+    x[:, 5] = 0.0
+    x[:, 600] = np.where(np.arange(6) < 3, -693.1, -693.2) * t
+    for kw in (dict(), dict(min_p=0.0)):
+        assert sample(lib, x, np.ones(6, np.float32), temperature=t, **kw).tolist() == [600] * 3 + [5] * 3
+
+
 @pytest.mark.parametrize("t", [4e35, 5e35, 7e35, 9e35, 2e36, 3e38])
 def test_sample_hot_rows_of_far_logits(lib, t):
     """Temperatures at which 693 t is at, or past, FP32's largest number, with logits over all of its range."""
