@@ -126,6 +126,16 @@ __device__ u64 block_scan(Shared& sh, u64 v) {
     return v + __shfl_sync(0xffffffffu, add, 0);
 }
 
+__device__ __forceinline__ double scan(double v) {   // inclusive, over the warp
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+    }
+    return v;
+}
+
 __device__ __forceinline__ void clear(Shared& sh) {
     for (int i = threadIdx.x; i < BINS; i += THREADS) sh.low[i] = sh.high[i] = 0;
     if (threadIdx.x == 0) sh.listed = 0;
@@ -272,10 +282,11 @@ __device__ bool finish_list(cg::cluster_group& cl, Shared& sh, Row& r, u64 befor
 }
 
 // The kept logits with in(x) are at most SMALL and hold all of the top k: the first CTA ranks them, cuts by k and p
-// and draws. Masses are fixed point, as the list's order is anybody's.
+// and draws. Top-p's masses are fixed point, as the list's order is anybody's; the draw's are FP64, in the order of the
+// indices: it may fall on a weight that is nothing next to the largest.
 template <typename In>
 __device__ void finish_small(cg::cluster_group& cl, Shared& sh, const Row& r, int k, double p, double u, int32_t* token, In in) {
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Shared* lead = cl.map_shared_rank(&sh, 0);
     for_kept(r, [&](float x, int i) {
         if (in(x)) put(r, lead, i, x, fixed_weight(r, x));
@@ -287,32 +298,42 @@ __device__ void finish_small(cg::cluster_group& cl, Shared& sh, const Row& r, in
     const u64 me = mine ? sh.list[tid] : 0, w = mine ? sh.list_mass[tid] : 0;
     const int index = (int)~(uint32_t)me;
     u64 ahead = 0;
-    int rank = 0;
+    int rank = 0, place = 0;   // by logit, by index
     if (mine)
-        for (int j = 0; j < n; j++)
-            if (sh.list[j] > me) { rank++; ahead += sh.list_mass[j]; }
+        for (int j = 0; j < n; j++) {
+            const u64 it = sh.list[j];
+            if (it > me) { rank++; ahead += sh.list_mass[j]; }
+            if ((uint32_t)it > (uint32_t)me) place++;
+        }
     bool keep = mine && rank < k;
-    auto sum = [&](u64 v) {
-        v = block_scan(sh, v);
-        if (tid == THREADS - 1) sh.total = v;
-        __syncthreads();
-        return sh.total;
-    };
     if (p < 1.0) {
-        const double target = fmax(p * (double)sum(keep ? w : 0), 0.5);
-        keep = keep && (double)ahead < target;
+        const u64 upto = block_scan(sh, keep ? w : 0);
+        if (tid == THREADS - 1) sh.total = upto;
+        __syncthreads();
+        keep = keep && (double)ahead < fmax(p * (double)sh.total, 0.5);
     }
-    const double target = u * (double)sum(keep ? w : 0);
     if (tid == 0) { sh.at = 0x7fffffff; sh.last = -1; }
-    if (mine && !keep) sh.list_mass[tid] = 0;
-    __syncthreads();
-    if (keep) {
-        u64 upto = 0;
-        for (int j = 0; j < n; j++)
-            if ((uint32_t)sh.list[j] >= (uint32_t)me) upto += sh.list_mass[j];   // indices up to this one
-        if (w && (double)upto > target) atomicMin(&sh.at, index);
-        atomicMax(&sh.last, index);
+    __syncthreads();   // the list has been read
+    double* weights = reinterpret_cast<double*>(sh.list_mass);
+    int* indices = reinterpret_cast<int*>(sh.list);
+    if (mine) {
+        weights[place] = keep ? weight(r, of_key((uint32_t)(me >> 32))) : 0.0;
+        indices[place] = index;
+        if (keep) atomicMax(&sh.last, index);
     }
+    __syncthreads();
+    const double here = mine ? weights[tid] : 0.0;
+    double upto = scan(here);
+    double* of_warp = reinterpret_cast<double*>(sh.warp_sum);
+    if (lane == 31) of_warp[warp] = upto;
+    __syncthreads();
+    double total = 0.0;
+#pragma unroll
+    for (int i = 0; i < SMALL / 32; i++) {
+        if (i < warp) upto += of_warp[i];
+        total += of_warp[i];
+    }
+    if (here > 0.0 && upto > u * total) atomicMin(&sh.at, indices[tid]);
     __syncthreads();
     if (tid == 0) *token = sh.at < 0x7fffffff ? sh.at : sh.last;
 }
@@ -414,15 +435,6 @@ __device__ bool cut(cg::cluster_group& cl, Shared& sh, Row& r, int k, double p, 
     }
 }
 
-__device__ __forceinline__ double scan(double v) {   // inclusive, over the warp
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const double x = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += x;
-    }
-    return v;
-}
 // v: inclusive sums by lane of what each lane has, if any; the first lane that has some and whose sum, behind `ahead`,
 // passes the target (32: none); ahead moves to its start. A sum's last bits depend on its order, so a lane without
 // weight may seem to pass.

@@ -93,6 +93,21 @@ def test_token_ranges_past_the_arrays(lib, start, tokens, reported):
 
 # ---- sampling ----------------------------------------------------------------------------------------------------
 
+def test_sample_small_weights_of_few_candidates(lib):
+    """Weights far below the largest count in the draw as the others do: u = 0 takes the first kept index that weighs anything."""
+    x = np.full((5, 700), -np.inf, np.float32)
+    x[0, [100, 200]] = -40.0, 0.0
+    x[1, [3, 4, 600]] = -35.0, -36.0, 0.0
+    x[2, [3, 4, 600]] = -35.0, -36.0, 0.0
+    x[3] = np.random.default_rng(1).permutation(np.linspace(0, -650, 700))
+    x[4, 50:60] = np.linspace(-300, 0, 10)
+    u = np.array([0.0, 5e-16, 7e-16, 0.0, 1e-38], np.float32)
+    for kw in (dict(top_k=5), dict(top_k=100), dict(top_k=200, min_p=1e-38), dict(top_k=150, top_p=1.0)):
+        want = [kvref.draw(x[i], float(u[i]), 1.0, kw["top_k"], 1.0, float(np.float32(kw.get("min_p", 0.0))))[0] for i in range(5)]
+        assert want[:3] == [100, 3, 4]
+        assert sample(lib, x, u, **kw).tolist() == want
+
+
 def test_sample_cut_at_2_to_the_minus_1000(lib):
     """Without filters and with one: a logit above 2^-1000 of the largest has a weight, one below has none."""
     t = np.array([0.5, 1.0, 3.0, 0.5, 1.0, 3.0], np.float32)
