@@ -155,6 +155,14 @@ __device__ __forceinline__ void split(float p0, float p1, uint32_t& hi, uint32_t
     lo = as_u32(__floats2half2_rn(p0 - f.x, p1 - f.y));
 }
 
+// A row's factor for its sums, in which V comes as value / 16; 0 for a row without a key. The unit is multiplied on after
+// it: 16 units may be more than FP32 holds, and a small one over L less than it holds in full.
+__device__ __forceinline__ float weighed(float L) { return L == 0.f ? 0.f : 16.f / L; }
+__device__ __forceinline__ void store4(float* to, float4 sum, float L, float unit) {
+    const float inv = weighed(L);
+    to[0] = sum.x * inv * unit; to[1] = sum.y * inv * unit; to[2] = sum.z * inv * unit; to[3] = sum.w * inv * unit;
+}
+
 // 16 log2(e) / sqrt(D) * k_unit = factor * 2^exponent, as its product with a row's power of two may leave FP32's range
 struct Scores {
     float factor;   // 0.5 .. 1
@@ -662,9 +670,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
             reinterpret_cast<float4*>(smem)[x] = acc;   // q's fragments are done with
             if (d == 0) cl_ml[c] = make_float2(M, L);
         } else if (parts == 1) {
-            const float inv = L == 0.f ? 0.f : 16.f * p.v_unit / L;   // V comes as value / 16
-            float* dst = out + row * D + d;
-            dst[0] = acc.x * inv; dst[1] = acc.y * inv; dst[2] = acc.z * inv; dst[3] = acc.w * inv;
+            store4(out + row * D + d, acc, L, p.v_unit);
         } else {
             const size_t at = row * sp.splits + split_id;
             *reinterpret_cast<float4*>(part_o + at * D + d) = acc;
@@ -695,9 +701,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
                 L += f * ml[r].y;
                 acc.x += f * v[r].x; acc.y += f * v[r].y; acc.z += f * v[r].z; acc.w += f * v[r].w;
             }
-        const float inv = L == 0.f ? 0.f : 16.f * p.v_unit / L;
-        float* dst = out + ((size_t)(first + ci / group) * hq + head * group + ci % group) * D + x % (D / 4) * 4;
-        dst[0] = acc.x * inv; dst[1] = acc.y * inv; dst[2] = acc.z * inv; dst[3] = acc.w * inv;
+        store4(out + ((size_t)(first + ci / group) * hq + head * group + ci % group) * D + x % (D / 4) * 4, acc, L, p.v_unit);
     }
     cl.sync();   // nobody leaves while its sums are read
 }
@@ -763,12 +767,12 @@ __global__ void __launch_bounds__(32 * JOIN) k_attn_paged_join(float* __restrict
     float L = 0.f;
 #pragma unroll
     for (int w = 0; w < JOIN; w++) L += sm_l[w];
-    const float inv = L == 0.f ? 0.f : 16.f * v_unit / L;
+    const float inv = weighed(L);
     for (int d = threadIdx.x; d < D; d += 32 * JOIN) {
         float acc = 0.f;
 #pragma unroll
         for (int w = 0; w < JOIN; w++) acc += sm_o[w][d];
-        out[row * D + d] = acc * inv;
+        out[row * D + d] = acc * inv * v_unit;
     }
 }
 

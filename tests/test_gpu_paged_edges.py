@@ -53,6 +53,20 @@ def test_attention_scores_scale(lib, dim, group, unit, top):
     check_scores(lib, dim, group, unit, top)
 
 
+@pytest.mark.parametrize("lens", [[40], [777], [9000]])   # one chunk, a cluster of them, two launches
+@pytest.mark.parametrize("unit", [3e37, 2e-38])
+def test_attention_value_unit(lib, lens, unit):
+    """Values next to FP32's largest and smallest normal numbers."""
+    c = Cache(lens, 1, 128, 16, (1.0, unit), seed=1)
+    fill_random(c, 3)
+    q = np.random.default_rng(4).standard_normal((1, 2, 128)).astype(np.float32)
+    out = attend(lib, c, c.batch(lens), q, 2).reshape(1, 2, 128)
+    k, v = c.kv(0, lens[0])
+    ref, size = kvref.attention(q, k, v, lens)
+    # the last product may fall among the subnormal numbers, which are 2^-149 apart
+    assert np.max(np.abs(out - ref)) <= tolerance(size, 128, np.abs(v).max(), lens[0]) + 2.0 ** -150
+
+
 # ---- token ranges ----------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("start,tokens,reported", [
