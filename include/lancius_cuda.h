@@ -52,7 +52,8 @@ lancius_error lcu_synchronize(lcu_ctx* ctx);     /* also reports device watchdog
  * (a bounded mbarrier wait that gave up) as LANCIUS_ERROR_INTERNAL, clearing it. The
  * per-op launchers that return before the work is done (lcu_attention, lcu_layernorm
  * ...) report trips here; the blocking ones (lcu_matmul, lcu_conv2d, the INT8 and
- * column-split GEMMs, lcu_matmul_noalloc) check before they return. */
+ * column-split GEMMs, lcu_matmul_noalloc) check before they return. Reports what the calls
+ * on the paged cache left out (see there) as LANCIUS_ERROR_SHAPE_MISMATCH; nothing else does. */
 lancius_error lcu_check_stream(void* stream);
 /* Test hook (no reference counterpart): launches a kernel whose bounded wait on an
  * mbarrier nothing arrives on gives up and sets the GEMM watchdog word, so the next

@@ -284,5 +284,5 @@ extern "C" lancius_error lcu_gemm_colsplit_fused(lcu_comm* comm, float* c, const
         if (r != ncclSuccess) return nccl_fail(r, "ncclAllGather (barrier)");
     }
     // the host record of the group table must stay valid until the copy ran
-    return lcu_check_stream(st);
+    return lcu_check_watchdogs(st);
 }

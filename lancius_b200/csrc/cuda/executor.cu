@@ -205,41 +205,57 @@ void lcu_ctx_retarget_schedule(lcu_ctx* c, lancius_schedule* s) {
     if (c && c->dmem) c->s = s;
 }
 
-// Waits for `stream`, then reads the tensor-core kernels' watchdog words of the current
-// device (set when a bounded mbarrier wait gave up): any set word is cleared and reported
-// as LANCIUS_ERROR_INTERNAL. The last words are the paged cache's (a page number or length out
-// of range), reported as LANCIUS_ERROR_SHAPE_MISMATCH unless a watchdog tripped too. The
-// words are per device, shared by every stream on it.
-lancius_error lcu_check_stream(void* stream) {
+// Waits for `stream`, then reads device words of the current device: clears those that are set and marks them in `set`.
+static lancius_error take_words(void* stream, int* const* words, bool* set, int n) {
     cudaStream_t st = lcu_as_stream(stream);
-    int* words[6] = {lcu_gemm_watchdog_addr(), lcu_attention_watchdog_addr(), lcu_conv_watchdog_addr(),
-                     lcu_int8_watchdog_addr(), lcu_kv_fault_addr(), lcu_attn_paged_fault_addr()};
     int vals[6] = {0, 0, 0, 0, 0, 0};
-    for (int i = 0; i < 6; i++)
+    for (int i = 0; i < n; i++)
         if (words[i]) {
             cudaError_t ce = cudaMemcpyAsync(&vals[i], words[i], sizeof(int), cudaMemcpyDeviceToHost, st);
             if (ce != cudaSuccess) return cuda_fail(ce);
         }
     cudaError_t ce = cudaStreamSynchronize(st);
     if (ce != cudaSuccess) return cuda_fail(ce);
-    bool tripped = false;
-    for (int i = 0; i < 6; i++)
-        if (vals[i] && words[i]) {
-            tripped = tripped || i < 4;
+    bool any = false;
+    for (int i = 0; i < n; i++)
+        if ((set[i] = vals[i] && words[i])) {
+            any = true;
             cudaMemsetAsync(words[i], 0, sizeof(int), st);
         }
-    if (tripped || vals[4] || vals[5]) {
-        cudaStreamSynchronize(st);
-        return fail(tripped ? LANCIUS_ERROR_INTERNAL : LANCIUS_ERROR_SHAPE_MISMATCH);
-    }
+    if (any) cudaStreamSynchronize(st);
     return LANCIUS_ERROR_OK;
 }
 
-// Waits for the context's stream and reports watchdog trips (lcu_check_stream).
+// Waits for `stream`, then reads the tensor-core kernels' watchdog words of the current
+// device (set when a bounded mbarrier wait gave up): any set word is cleared and reported
+// as LANCIUS_ERROR_INTERNAL. The words are per device, shared by every stream on it.
+lancius_error lcu_check_watchdogs(void* stream) {
+    int* const words[4] = {lcu_gemm_watchdog_addr(), lcu_attention_watchdog_addr(), lcu_conv_watchdog_addr(),
+                           lcu_int8_watchdog_addr()};
+    bool set[4];
+    lancius_error e = take_words(stream, words, set, 4);
+    if (e != LANCIUS_ERROR_OK) return e;
+    return set[0] || set[1] || set[2] || set[3] ? fail(LANCIUS_ERROR_INTERNAL) : LANCIUS_ERROR_OK;
+}
+
+// As above, and reads the paged cache's words (a page number, length or token range out of
+// bounds), reported as LANCIUS_ERROR_SHAPE_MISMATCH unless a watchdog tripped too. The calls that
+// check their own work do not read these: they would fail for, and take away, another call's report.
+lancius_error lcu_check_stream(void* stream) {
+    int* const words[6] = {lcu_gemm_watchdog_addr(), lcu_attention_watchdog_addr(), lcu_conv_watchdog_addr(),
+                           lcu_int8_watchdog_addr(), lcu_kv_fault_addr(), lcu_attn_paged_fault_addr()};
+    bool set[6];
+    lancius_error e = take_words(stream, words, set, 6);
+    if (e != LANCIUS_ERROR_OK) return e;
+    if (set[0] || set[1] || set[2] || set[3]) return fail(LANCIUS_ERROR_INTERNAL);
+    return set[4] || set[5] ? fail(LANCIUS_ERROR_SHAPE_MISMATCH) : LANCIUS_ERROR_OK;
+}
+
+// Waits for the context's stream and reports watchdog trips (lcu_check_watchdogs).
 lancius_error lcu_synchronize(lcu_ctx* c) {
     if (!c) return fail(LANCIUS_ERROR_NULL_PTR);
     cudaSetDevice(c->device);
-    return lcu_check_stream(c->stream);
+    return lcu_check_watchdogs(c->stream);
 }
 
 int lcu_last_launch_count(lcu_ctx* c) { return c ? c->last_launches : 0; }

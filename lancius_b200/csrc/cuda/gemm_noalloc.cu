@@ -114,6 +114,6 @@ extern "C" lancius_error lcu_matmul_noalloc(float* out, const float* a, const fl
     lancius_error e = lcu_gemm_tc_prepare(&p, scratch, M, N, K, 1, 1, 1, passes);
     if (e == LANCIUS_ERROR_OK) e = lcu_gemm_tc_run(&p, d_group, epilogue, stream);
     // `h` lives on this stack frame: wait until the copy (and the GEMM) ran
-    lancius_error se = lcu_check_stream(st);
+    lancius_error se = lcu_check_watchdogs(st);
     return e != LANCIUS_ERROR_OK ? e : se;
 }

@@ -180,6 +180,6 @@ int lcu_attention_watchdog_read_and_clear(void);
 void lcu_reset_launch_count(void);
 int lcu_launch_count(void);
 // cudaStreamSynchronize + report (and clear) tensor-core watchdog trips as LANCIUS_ERROR_INTERNAL
-lancius_error lcu_check_stream(void* stream);
+lancius_error lcu_check_watchdogs(void* stream);
 void lcu_ctx_retarget_schedule(lcu_ctx* c, lancius_schedule* s);
 }

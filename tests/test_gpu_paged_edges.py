@@ -105,6 +105,23 @@ def test_token_ranges_past_the_arrays(lib, start, tokens, reported):
         assert (q[t] == 7.0).all() and (out[t] == 7.0).all() and (ko[t] == 7.0).all()
 
 
+def test_bad_pages_are_not_other_calls_faults(lib):
+    """A bad page is reported by lcu_check_stream, and neither fails nor vanishes in calls that check their own work."""
+    c = Cache([40], 1, 64, 16)
+    c.table[0, 2] = -1
+    x = np.random.default_rng(1).standard_normal((1, 3 * 64)).astype(np.float32)
+    append(lib, c, c.batch([40]), x, 1)
+    n = 256
+    a = torch.randn((n, n), device="cuda")
+    y = torch.empty((n, n), device="cuda")
+    ctx = lib.lcu_create(0)
+    assert ctx
+    assert lib.lcu_synchronize(ctx) == 0
+    lib.lcu_destroy(ctx)
+    assert lib.lcu_matmul(ptr(y), ptr(a), ptr(a), n, n, n, None, 0, 0, None) == 0
+    assert lib.lcu_check_stream(None) == SHAPE and lib.lcu_check_stream(None) == 0
+
+
 # ---- sampling ----------------------------------------------------------------------------------------------------
 
 def test_sample_small_weights_of_few_candidates(lib):
