@@ -60,6 +60,7 @@ constexpr float RAISE = 8.f;      // the running maximum moves only when exceede
 constexpr float FAR = 4194304.f;
 
 __device__ int g_attn_paged_fault = 0;
+std::atomic<bool> g_used{false};   // a kernel of this file has been launched: before that the word needs no reading
 
 template <int D, int ROWS>   // ROWS of q per CTA: 4 or a multiple of 8
 struct Shape {
@@ -896,6 +897,7 @@ extern "C" {
 
 int* lcu_attn_paged_fault_addr(void) {
     void* p = nullptr;
+    if (!g_used.load(std::memory_order_relaxed)) return nullptr;
     return cudaGetSymbolAddress(&p, g_attn_paged_fault) == cudaSuccess ? static_cast<int*>(p) : nullptr;
 }
 
@@ -930,6 +932,7 @@ lancius_error lcu_attention_paged(float* out, const float* q, size_t q_ld, size_
         part_ml = reinterpret_cast<float2*>(part_o + rows * D);
     }
     cudaStream_t st = lcu_as_stream(stream);
+    g_used.store(true, std::memory_order_relaxed);
     return with_shape((int)D, hq / p.heads * b.max_new,
                       [&](auto d, auto n) {
                           if constexpr (n <= 8)

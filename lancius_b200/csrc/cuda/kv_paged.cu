@@ -25,6 +25,7 @@ namespace {
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 
 __device__ int g_kv_fault = 0;
+std::atomic<bool> g_used{false};   // a kernel of this file has been launched: before that the word needs no reading
 
 // Where one warp works: token, sequence, position, and the cache row of (token, head 0) or -1.
 struct Place {
@@ -305,6 +306,7 @@ extern "C" {
 
 int* lcu_kv_fault_addr(void) {
     void* p = nullptr;
+    if (!g_used.load(std::memory_order_relaxed)) return nullptr;
     return cudaGetSymbolAddress(&p, g_kv_fault) == cudaSuccess ? static_cast<int*>(p) : nullptr;
 }
 
@@ -330,6 +332,7 @@ lancius_error lcu_kv_append_paged(const lcu_kv_pages* pages, const lcu_kv_batch*
     const unsigned grid = part_blocks(b.n_tokens, shift);
     cudaStream_t st = lcu_as_stream(stream);
     auto kernel = D == 64 ? k_kv_append<64> : D == 128 ? k_kv_append<128> : k_kv_append<256>;
+    g_used.store(true, std::memory_order_relaxed);
     kernel<<<grid, THREADS, 0, st>>>(p, b, shift, q_out, q, q_ld, hq, k, k_ld, v, v_ld, lb, rotate, wide);
     lcu_note_launch();
     return lcu_launch_status();
@@ -347,6 +350,7 @@ lancius_error lcu_kv_read_paged(float* k_out, float* v_out, const lcu_kv_pages* 
     const int shift = part_shift(b.n_tokens, 2 * p.heads, 256 / (int)D);
     const int wide = min(width(k_out, 0), width(v_out, 0));
     auto kernel = D == 64 ? k_kv_read<64> : D == 128 ? k_kv_read<128> : k_kv_read<256>;
+    g_used.store(true, std::memory_order_relaxed);
     kernel<<<part_blocks(b.n_tokens, shift), THREADS, 0, lcu_as_stream(stream)>>>(k_out, v_out, p, b, shift, wide);
     lcu_note_launch();
     return lcu_launch_status();

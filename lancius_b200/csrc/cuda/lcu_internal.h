@@ -156,7 +156,7 @@ int* lcu_attention_watchdog_addr(void);
 int* lcu_conv_watchdog_addr(void);
 int* lcu_int8_watchdog_addr(void);
 int* lcu_gemm_watchdog_addr(void);
-// set by the paged-cache kernels when a page number or a length was out of range
+// set by the paged-cache kernels when a page number or a length was out of range; NULL before their first launch
 int* lcu_kv_fault_addr(void);
 int* lcu_attn_paged_fault_addr(void);
 void* lcu_scratch_acquire_gather(size_t bytes);

@@ -1,9 +1,14 @@
 """The paged cache, its attention and the sampler where numbers, lengths and bounds end: units and queries whose product
 leaves FP32's range, token ranges that do not fit, weights far below the largest, the longest sequences, prompts."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
 import kvref
+import lancius_b200 as L
 from test_gpu_paged import BASE, SHAPE, Cache, append, attend, check_sample, fill_random, lib, ptr, sample, tolerance  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -120,6 +125,28 @@ def test_bad_pages_are_not_other_calls_faults(lib):
     lib.lcu_destroy(ctx)
     assert lib.lcu_matmul(ptr(y), ptr(a), ptr(a), n, n, n, None, 0, 0, None) == 0
     assert lib.lcu_check_stream(None) == SHAPE and lib.lcu_check_stream(None) == 0
+
+
+def test_words_are_read_only_after_a_launch(lib):
+    """A program that never calls the paged cache does not load its kernels for lcu_check_stream, nor wait for its words."""
+    code = """
+import ctypes as C, torch, lancius_b200 as L
+lib = L.load()
+for name in ("lcu_kv_fault_addr", "lcu_attn_paged_fault_addr"):
+    f = getattr(lib, name)
+    f.restype, f.argtypes = C.c_void_p, []
+    assert lib.lcu_check_stream(None) == 0 and f() is None, name
+from test_gpu_paged import Cache, append, attend
+import numpy as np
+c = Cache([40], 1, 64, 16)
+append(lib, c, c.batch([40]), np.ones((1, 192), np.float32), 1)
+assert lib.lcu_kv_fault_addr() and lib.lcu_attn_paged_fault_addr() is None
+attend(lib, c, c.batch([40]), np.ones((1, 64), np.float32), 1)
+assert lib.lcu_attn_paged_fault_addr()
+"""
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join((os.path.dirname(here), here)))
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, env=env)
 
 
 # ---- sampling ----------------------------------------------------------------------------------------------------
