@@ -175,6 +175,8 @@ struct Split {
     bool cluster;   // k_attn_paged's CLUSTER
 };
 
+__device__ __forceinline__ int chunks_of(int keys, int chunk) { return keys / chunk + (keys % chunk != 0); }
+
 // CLUSTER: the splits of a block of rows are a cluster, whose CTAs join their sums without another kernel
 template <int D, int ROWS, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, Shape<D, ROWS>::RESIDENT)
@@ -202,7 +204,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     const int keys = min(max(len, 0), b.max_len);
     if (split_id == 0 && block == 0 && tid == 0 && (len > b.max_len || count > b.max_new || !whole)) g_attn_paged_fault = 1;
     const int cols = min(COLS, used * group - block * COLS);     // rows of this block
-    const int parts = max(1, (keys + sp.chunk - 1) / sp.chunk);   // chunks of this sequence
+    const int parts = max(1, chunks_of(keys, sp.chunk));          // of this sequence
     if (cols <= 0 || split_id >= parts) {
         if (CLUSTER && cols > 0 && parts > 1) {   // the others' barriers
             cg::this_cluster().sync();
@@ -223,7 +225,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
 #pragma unroll
     for (int r = 0; r < R; r++) limit[r] = limit_of(row_at(r));
     least = limit_of(0);                                          // positions rise with the row
-    const int begin = split_id * sp.chunk, end = min(begin + sp.chunk, limit_of(cols - 1));
+    const int begin = split_id * sp.chunk, end = begin + min(sp.chunk, limit_of(cols - 1) - begin);
 
     // q: a lane takes 8 channels, on their way while the first tiles are asked for
     constexpr int LANES = D / 8, QC = (COLS * LANES + THREADS - 1) / THREADS;   // lanes of a row, rows of a lane
@@ -255,8 +257,8 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
     const int slot_mask = (1 << p.page_shift) - 1;
     const uint32_t heads = p.heads;
     auto row_of = [&](int i) {   // cache row of this lane's key of tile i, NONE: no key, or no such page
-        const int key = begin + TILE * (warp + WARPS * i) + lane;
-        if (i >= tiles || key >= end) return NONE;
+        const uint32_t key = (uint32_t)begin + TILE * (warp + WARPS * i) + lane;
+        if (i >= tiles || key >= (uint32_t)end) return NONE;
         const int page = table[key >> p.page_shift];
         if (page >= 0 && page < p.n_pages) return (((uint32_t)page * heads + head) << p.page_shift) + (key & slot_mask);
         g_attn_paged_fault = 1;
@@ -505,7 +507,7 @@ k_attn_paged(float* __restrict__ out, const float* __restrict__ q, size_t q_ld, 
         for (int r = 0; r < R; r++)
 #pragma unroll
             for (int x = 0; x < X; x++) sv[r][x] = a[r >> 1][x >> 1][2 * (x & 1) + (r & 1)];   // times cs[r]: log2 units
-        if (key0 + TILE > least) {
+        if (key0 > least - TILE) {
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
@@ -720,7 +722,7 @@ __global__ void __launch_bounds__(32 * JOIN) k_attn_paged_join(float* __restrict
     const int s = blockIdx.z, i = blockIdx.y, h = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int first, count, behind;
     kv_new_tokens(b, s, first, count, behind);
-    const int keys = min(max(b.seq_len[s], 0), b.max_len), parts = (keys + sp.chunk - 1) / sp.chunk;
+    const int keys = min(max(b.seq_len[s], 0), b.max_len), parts = chunks_of(keys, sp.chunk);
     asm volatile("griddepcontrol.wait;" ::: "memory");   // also before an early return: the next kernel waits for this one only
     if (i >= count || parts <= 1) return;
     const size_t row = (size_t)(first + i) * hq + h;

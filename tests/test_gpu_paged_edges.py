@@ -9,7 +9,7 @@ import pytest
 
 import kvref
 import lancius_b200 as L
-from test_gpu_paged import BASE, SHAPE, Cache, append, attend, check_sample, fill_random, lib, ptr, sample, tolerance  # noqa: F401
+from test_gpu_paged import BASE, SHAPE, Cache, append, attend, check_sample, fill_random, i32, lib, ptr, sample, tolerance  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -147,6 +147,29 @@ assert lib.lcu_attn_paged_fault_addr()
     here = os.path.dirname(os.path.abspath(__file__))
     env = dict(os.environ, PYTHONPATH=os.pathsep.join((os.path.dirname(here), here)))
     subprocess.run([sys.executable, "-c", code], check=True, timeout=300, env=env)
+
+
+# ---- the longest sequences, prompts ----------------------------------------------------------------------------
+
+def test_attention_next_to_31_bits(lib):
+    """The longest sequence that a table can describe: all of its entries name one of two pages."""
+    page, width = 16, (2 ** 31 - 1) // 16
+    c = Cache([32], 1, 64, page, spare=0)
+    n = page * width - 3
+    c.kc.fill_(0x88)                 # keys of zero: equal weights
+    c.ks.fill_(0x38)
+    c.vs.fill_(0x38)
+    c.vc[0].fill_(0x99)              # 1
+    c.vc[1].fill_(0x77)              # -1
+    table = torch.ones(width, dtype=torch.int32, device="cuda")
+    table[:width // 4] = 0
+    lens = i32([n])
+    b = L.KvBatch(ptr(table), width, ptr(lens), None, 1, 1, 0, 0)
+    out = attend(lib, c, b, np.ones((1, 64), np.float32), 1)
+    assert lib.lcu_check_stream(None) == 0
+    first = page * (width // 4)
+    # sums of up to 2^21 chunks of equal weight: every one but the last chunk's is a whole number below 2^24 times 2^15
+    assert np.max(np.abs(out - (first - (n - first)) / n)) <= 2.0 ** -20
 
 
 # ---- sampling ----------------------------------------------------------------------------------------------------
