@@ -9,7 +9,8 @@ import pytest
 
 import kvref
 import lancius_b200 as L
-from test_gpu_paged import BASE, SHAPE, Cache, append, attend, check_sample, fill_random, i32, lib, ptr, sample, tolerance  # noqa: F401
+from test_gpu_paged import (BASE, SHAPE, Cache, append, attend, check_sample, fill_random, i32, lib, ptr, sample,  # noqa: F401
+                            tolerance)
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -170,6 +171,19 @@ def test_attention_next_to_31_bits(lib):
     first = page * (width // 4)
     # sums of up to 2^21 chunks of equal weight: every one but the last chunk's is a whole number below 2^24 times 2^15
     assert np.max(np.abs(out - (first - (n - first)) / n)) <= 2.0 ** -20
+
+
+def test_attention_workspace_refusals(lib):
+    """A call that needs a workspace refuses none, a short one and an unaligned one."""
+    c = Cache([9000], 1, 64, 16)
+    b = c.batch([9000])
+    q = torch.zeros((1, 64), device="cuda")
+    need = lib.lcu_attention_paged_workspace(c.pages, b, 1)
+    assert need > 0
+    space = torch.empty(need + 16, dtype=torch.uint8, device="cuda")
+    assert lib.lcu_attention_paged(ptr(q), ptr(q), 64, 1, c.pages, b, ptr(space), need - 1, None) == -9
+    assert lib.lcu_attention_paged(ptr(q), ptr(q), 64, 1, c.pages, b, None, need, None) == -2
+    assert lib.lcu_attention_paged(ptr(q), ptr(q), 64, 1, c.pages, b, ptr(space) + 8, need, None) == -5
 
 
 # ---- sampling ----------------------------------------------------------------------------------------------------
