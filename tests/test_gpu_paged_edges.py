@@ -9,7 +9,7 @@ import pytest
 
 import kvref
 import lancius_b200 as L
-from test_gpu_paged import (BASE, SHAPE, Cache, append, attend, check_sample, fill_random, i32, lib, ptr, sample,  # noqa: F401
+from test_gpu_paged import (BASE, SHAPE, Cache, append, attend, check_sample, fill_random, i32, lib, ptr, sample, starts,  # noqa: F401
                             tolerance)
 
 pytestmark = pytest.mark.gpu
@@ -171,6 +171,31 @@ def test_attention_next_to_31_bits(lib):
     first = page * (width // 4)
     # sums of up to 2^21 chunks of equal weight: every one but the last chunk's is a whole number below 2^24 times 2^15
     assert np.max(np.abs(out - (first - (n - first)) / n)) <= 2.0 ** -20
+
+
+@pytest.mark.parametrize("dim,heads,group,lens,new", [
+    (64, 2, 4, [2500, 100], [2500, 1]),
+    (128, 2, 4, [2000, 333, 700, 1], [1500, 1, 1, 1]),          # a prompt beside single tokens
+    (256, 1, 2, [1300, 1900], [1, 1200])])
+def test_attention_prompts(lib, dim, heads, group, lens, new):
+    """More than a thousand new tokens in a call, over several chunks of keys."""
+    hq = heads * group
+    c = Cache(lens, heads, dim, 32, seed=6)
+    fill_random(c, 7)
+    q = np.random.default_rng(8).standard_normal((sum(new), hq, dim)).astype(np.float32)
+    out = torch.from_numpy(attend(lib, c, c.batch(lens, starts(new), max_new=max(new)), q, hq).reshape(-1, hq, dim)).cuda().double()
+    assert lib.lcu_check_stream(None) == 0
+    at = 0
+    for s, (n, m) in enumerate(zip(lens, new)):
+        k, v = (torch.from_numpy(a).cuda().repeat_interleave(group, 1) for a in c.kv(s, n))
+        x = torch.from_numpy(q[at:at + m]).cuda().double()
+        size = torch.einsum("nhd,khd->nhk", x.abs(), k.abs()).max().item() / dim ** 0.5
+        z = torch.einsum("nhd,khd->nhk", x, k) / dim ** 0.5
+        limit = torch.arange(n - m, n, device="cuda")
+        z = z.masked_fill(torch.arange(n, device="cuda") > limit[:, None, None], -np.inf)
+        ref = torch.einsum("nhk,khd->nhd", z.softmax(2), v)
+        assert (out[at:at + m] - ref).abs().max().item() <= tolerance(size, dim, v.abs().max().item(), n)
+        at += m
 
 
 def test_attention_workspace_refusals(lib):
