@@ -228,8 +228,9 @@ lancius_error lcu_conv2d_bwd_w(float* out, const float* grad, const float* in, s
  * Cache format: 4-bit codes n = 1 .. 15 for the numbers v = n - 8 in groups of 16 channels
  * with one e4m3 scale byte each; value = v * scale * unit. Channel 2i of a row is the low
  * nibble of byte i. scale = e4m3(max|x| / (7 unit)), v = x / (scale * unit), both rounded to the
- * nearest, ties to even, v held within -7 .. 7. A group that holds a NaN or an infinity gets
- * the scale NaN (0x7f). Reading takes any code (0 is -8) and any non-negative scale. */
+ * nearest, ties to even, v held within -7 .. 7, where x / unit is first rounded to FP32 (no change for
+ * a unit of 1). A group in which that gives a NaN or an infinity gets the scale NaN (0x7f). Reading
+ * takes any code (0 is -8) and any non-negative scale. */
 typedef struct {
     uint8_t* k_codes;      /* [n_pages][n_heads][page_size][head_dim / 2], 16-byte aligned */
     uint8_t* v_codes;
@@ -250,7 +251,8 @@ typedef struct {
  * left as they were, as is the cache for them. Rows that token_start places before row 0 or at and
  * after n_tokens do not exist: they are left out, which lcu_check_stream then reports as
  * LANCIUS_ERROR_SHAPE_MISMATCH, and the sequence's other rows keep their positions. A token whose position is negative (an idle
- * slot with seq_len 0) is not appended, and its attention row is zero. */
+ * slot with seq_len 0) is not appended, its rows of q_out, k_out and v_out are left as they were, and its
+ * attention row is zero. */
 typedef struct {
     const int32_t* page_table;    /* device, [n_seqs][table_width] */
     size_t table_width;
@@ -280,12 +282,19 @@ lancius_error lcu_kv_read_paged(float* k_out, float* v_out, const lcu_kv_pages* 
                                 void* stream);
 /* out[t][h] = softmax(q[t][h] . K / sqrt(head_dim)) V over keys 0 .. position of row t; query
  * head h reads key head h / (n_q_heads / n_heads). q rows q_ld floats apart, out
- * [n_tokens][n_q_heads * head_dim]. workspace: lcu_attention_paged_workspace() bytes (0 where
- * the keys are few), 16-byte aligned, used by this call alone until it has run (two captured
- * graphs that may run at the same time need two). A NaN or infinity in the cache shows only in the rows that see it: a
- * row that sees one in a value is NaN in all its channels. Pages outside the cache count as zeros; they, and
- * lengths over max_seq_len or max_new, are reported as above (the keys and rows over the
- * bound are left out). */
+ * [n_tokens][n_q_heads * head_dim].
+ * Precision: q and the weights have 22 bits (two 16-bit halves each), keys and values all of theirs, sums
+ * are FP32; a weight below 2^-32 of the largest adds to the sum of the weights only. Against 64 bits the
+ * result is off by 3e-7 to 1e-6 of its size, as a plain FP32 form's is.
+ * workspace: lcu_attention_paged_workspace() bytes (0 where the keys are few), 16-byte aligned, used by this
+ * call alone until it has run (two captured graphs that may run at the same time need two). It is
+ * n_tokens * n_q_heads * (head_dim + 2) floats for every chunk of up to 2048 keys (1280 for heads of 256):
+ * 3.5 GB for 8192 new tokens of 32768 with 32 heads of 128, so give a long prompt in pieces of some hundred
+ * tokens. The grid has room for max_new tokens in every sequence, so prompts and single tokens are faster
+ * in two calls than in one.
+ * A NaN or infinity in the cache shows only in the rows that see it: a row that sees one in a value is NaN
+ * in all its channels. Pages outside the cache count as zeros; they, and lengths over max_seq_len or
+ * max_new, are reported as above (the keys and rows over the bound are left out). */
 lancius_error lcu_attention_paged(float* out, const float* q, size_t q_ld, size_t n_q_heads, const lcu_kv_pages* pages,
                                   const lcu_kv_batch* batch, void* workspace, size_t workspace_bytes, void* stream);
 size_t lcu_attention_paged_workspace(const lcu_kv_pages* pages, const lcu_kv_batch* batch, size_t n_q_heads);

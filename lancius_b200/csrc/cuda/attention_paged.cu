@@ -6,15 +6,18 @@
 // Bound: the floor is HBM. A key/value pair of one head is D + D / 8 bytes and is read once for all rows of its key
 // head ((new token, query head) pairs, up to 24 per CTA); at the measured copy rate an SM receives about 46 codes a
 // clock, so turning codes into operands is the work that has to fit beside the loads. What bounds the kernel is the
-// issue of that work: 760 instructions a warp and tile of 32 keys of 128 with up to 4 rows, 800 with 8, in which the
-// tensor pipe is busy for 21 and 38 %. Four warps a quarter of an SM issue them at nine tenths of the rate within the
-// loop, at 61 % over the kernel, as a CTA spends a quarter of its time on lengths, first loads and its merge. MMAs
+// issue of that work: 770 instructions a warp and tile of 32 keys of 128 with up to 4 rows, 805 with 8, in which the
+// tensor pipe is busy for 20 and 38 %. Four warps a quarter of an SM issue them at nine tenths of the rate within the
+// loop, at 60 to 62 % over the kernel, as a CTA spends a quarter of its time on lengths, first loads and its merge. MMAs
 // do not overlap with the half-rate LOP3 and HFMA2 (18.3 clocks for a group with its MMA, 9.5 without).
-//   131072 keys of one sequence, 8 key heads of 128, 4 rows each: 41.0 us, 3.7 TB/s (0.56 of the measured copy rate)
-//   32 sequences of up to 8192 keys, 8 key heads of 128, one row each: 66.4 us, 3.55 TB/s (0.54)
-//   64 sequences of up to 8000 keys, 8 key heads of 128, 8 rows each: 133 us, 3.4 TB/s (0.51); the loads alone 83 us
+//   131072 keys of one sequence, 8 key heads of 128, 4 rows each: 40.8 us, 3.7 TB/s (0.57 of the measured copy rate)
+//   32 sequences of up to 8192 keys, 8 key heads of 128, one row each: 66.5 us, 3.55 TB/s (0.54)
+//   64 sequences of up to 8000 keys, 8 key heads of 128, 8 rows each: 137 us, 3.3 TB/s (0.50); the loads alone 83 us
 //   24 sequences of up to 3001 keys, 4 key heads of 64, 20 rows each: 19.5 us
-//   16 sequences of up to 5000 keys, one key head of 256, 8 rows: 12.9 us
+//   16 sequences of up to 5000 keys, one key head of 256, 8 rows: 12.4 us
+// Prompts run through the same kernel, 24 rows (16 of heads of 256) at a time, each of which reads the keys that they see and
+// turns them into operands again: 8192 new tokens of 8192, 32 heads on 8 of 128, take 4.6 ms, 121 TFLOP/s. The
+// shapes of 16 rows spill 140 (heads of 128) and 212 bytes (256) a thread.
 //
 // Products run as mma.sync m16n8k16 (f16 in, FP32 out). Measured 0.5 of them per clock and SM; two serve 256 codes
 // and 8 rows, so 64 codes a clock, above the HBM rate. tcgen05 would need the operands written to shared or tensor
@@ -25,8 +28,9 @@
 // fit (with q and p as A, halves stacked in its 16 rows, it took 160 registers and 63.4 us for the first of these, and
 // 60.0 with the codes as A at the same stage). Up to 4 rows put both halves into one operand: 47.7.
 //
-// Dequantising: a code or'ed into the mantissa of an f16 constant, then one HFMA2 with the group's factor and offset
-// gives (n - 8) scale / 16 without rounding (scale_of). Eight codes take 5 integer and 4 HFMA2 instructions. (4-bit
+// Dequantising, a known way for 4-bit weights (Kim et al., "Who Says Elephants Can't Run", 2022): a code or'ed into the
+// mantissa of an f16 constant, then one HFMA2 with the group's factor and offset gives (n - 8) scale / 16 without
+// rounding (scale_of). Eight codes take 5 integer and 4 HFMA2 instructions. (4-bit
 // floating point needs cvt, measured 25 codes a clock and SM, or more shifts.)
 //   S^T = K Q^T: A = K wants channel pairs of one key: a thread holds D / 4 contiguous channels of a key, any order of
 //     channels will do if q's fragment has the same.

@@ -7,14 +7,14 @@
 // over order-preserving 32-bit keys narrows it down to one key first. The draw adds weights in index order.
 //
 // Masses of bins are 64-bit fixed point, so the order of the atomics does not matter: 2^44 for the largest weight, and
-// 2^18 tokens fit 62 bits. The draw's sums are FP64 in a fixed order. Weights are FP64: with FP32 ones a drawn token
-// would differ from the exact one in about one row of a thousand.
+// 2^18 tokens fit 62 bits. The draw's sums are FP64 in a fixed order, on every path. Weights are FP64: with
+// FP32 ones a drawn token would differ from the exact one in about one row of a thousand.
 //
 // k_sample: a row is spread over a cluster of 1 to 8 CTAs that hold it in shared memory through all passes and exchange
 // histograms and sums through each other's shared memory; HBM is read once. Bound by the passes' instructions and by
 // the chain of barriers between them, not by HBM: of 29 us that a cluster needs for a quarter of 50021 logits a CTA with top-p,
 // the load takes 4, the histogram 8, its scan 3, the list 3, the ranking 1, the draw's weights 6, the draw 1.
-// 32000 logits with every filter: 8.3 us; 200 x 50021 with mixed filters: 55.3 us (top-p alone 84, top-k of 50 alone 34).
+// 32000 logits with every filter: 8.0 us; 200 x 50021 with mixed filters: 54 us (top-p alone 84, top-k of 50 alone 34).
 // k_sample_open, without filters: one pass, no part of the row kept. 64 x 131072: 20.6 us, of which the loads and
 // barriers alone take 9 (as greedy rows measure them) and the FP64 pipe is busy for 6: 12 instructions a logit.
 #include "lcu_internal.h"
@@ -487,8 +487,8 @@ __device__ __forceinline__ int draw_in_part(double mine, bool mine_any, int per,
     return __shfl_sync(0xffffffffu, block * BLOCK + 4 * lane + drawn, at);
 }
 
-// RESIDENT CTAs per SM: 3 take 40 registers a thread and some spills, which pays as soon as there are more CTAs than 2 per SM
-// hold (200 x 50021, mixed filters: 56.5 us, with 2 62.8; one row of 32000: 9.9 and 9.7)
+// RESIDENT CTAs per SM: 3 take 40 registers a thread and spill 464 bytes of it, which pays as soon as there are more CTAs than
+// 2 per SM hold (when first measured, 200 x 50021, mixed filters: 56.5 us, with 2 62.8; one row of 32000: 9.9 and 9.7)
 template <int RESIDENT>
 __global__ void __launch_bounds__(THREADS, RESIDENT) k_sample(int32_t* __restrict__ token, const float* __restrict__ logits, size_t ld,
                                                               int vocab, int part, int vec, const float* temperature,
