@@ -285,7 +285,7 @@ lancius_error lcu_kv_read_paged(float* k_out, float* v_out, const lcu_kv_pages* 
  * [n_tokens][n_q_heads * head_dim].
  * Precision: q and the weights have 22 bits (two 16-bit halves each), keys and values all of theirs, sums
  * are FP32; a weight below 2^-32 of the largest adds to the sum of the weights only. Against 64 bits the
- * result is off by 3e-7 to 1e-6 of its size, as a plain FP32 form's is.
+ * result is off by 3e-7 to 1.2e-6 of its size, as a plain FP32 form's is.
  * workspace: lcu_attention_paged_workspace() bytes (0 where the keys are few), 16-byte aligned, used by this
  * call alone until it has run (two captured graphs that may run at the same time need two). It is
  * n_tokens * n_q_heads * (head_dim + 2) floats for every chunk of up to 2048 keys (1280 for heads of 256):
@@ -309,7 +309,7 @@ size_t lcu_attention_paged_workspace(const lcu_kv_pages* pages, const lcu_kv_bat
  * A weight below 2^-1000 of the largest counts as zero. temperature <= 0 or NaN takes the
  * largest logit, the lowest index among equals. NaN logits count as -infinity; a row that has
  * nothing above -infinity gives -1. Masses are summed in 64 bits and do not depend on the
- * order in which the GPU runs. */
+ * order in which the GPU runs; those of top_p are whole multiples of 2^-44 of the largest weight. */
 lancius_error lcu_sample(int32_t* token, const float* logits, size_t ld, size_t rows, size_t vocab,
                          const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                          const float* u, void* stream);
